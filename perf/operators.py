@@ -413,7 +413,7 @@ def _plain_append_one(codes, scale, rows, slots, is_v):
     block, off = slots // PAGE, slots % PAGE
     top = rows.float().abs().amax(2) / 448
     m, e = torch.frexp(top)
-    e = (e - (m == 0.5).to(e.dtype)).clamp(min=LEAST)
+    e = torch.where(top > 0, e - (m == 0.5).to(e.dtype), LEAST).clamp(min=LEAST)
     old = torch.frexp(scale)[1] - 1
     fresh = torch.zeros(codes.shape[0], dtype=torch.bool, device=codes.device)
     fresh[block[off == 0]] = True
