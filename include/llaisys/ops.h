@@ -145,6 +145,88 @@ __C {
     __export void llaisysPagedAttentionVarlen(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool,
                                               llaisysTensor_t v_pool, llaisysTensor_t block_table,
                                               llaisysTensor_t cu_q, llaisysTensor_t ctx_len, float scale);
+
+    /* New; no counterpart in the reference. A step's tables from the requests'
+     * lengths, so that a serving loop's steps need no host work on them.
+     * Sequence b holds ctx_len[b] tokens and gets new_len[b]: [B] I32 each.
+     *   cu_new [B+1] I32: prefix sums of new_len (negative: 0), at most T.
+     *   block_table [B, max_pages] I32, updated in place: the pages that the new
+     *     tokens begin get blocks from free_blocks [F] I32, from free_used[0]
+     *     on, in the order of the sequences and pages; free_after[0] is
+     *     free_used[0] plus the blocks taken ([1] I32 each). All three NULL:
+     *     every page is mapped already.
+     *   ctx_after [B] I32: ctx_len + new_len.
+     *   pos_ids, slots [T] I64: row cu_new[b] + i is token ctx_len[b] + i of
+     *     sequence b: its position, and block * 16 + offset, the place that
+     *     llaisysPagedKVAppendF8 writes. Rows behind the last sequence: position
+     *     0 and slot -1.
+     * A sequence is left as it is (ctx_after = ctx_len, no blocks, its rows as
+     * those behind the last sequence) if its lengths are negative or pass the
+     * table or its rows pass T (error bit 2), if the page its first row
+     * continues is not mapped (bit 1), or if free_blocks does not reach for it:
+     * then no later sequence takes blocks either (bit 8). A row whose page is
+     * not mapped gets position 0 and slot -1 (bit 1). ctx_after may be ctx_len
+     * itself and free_after free_used; T, F, B, max_pages under 2^30. */
+    __export void llaisysPagedKVMap(llaisysTensor_t block_table, llaisysTensor_t cu_new, llaisysTensor_t ctx_after,
+                                    llaisysTensor_t pos_ids, llaisysTensor_t slots, llaisysTensor_t ctx_len,
+                                    llaisysTensor_t new_len, llaisysTensor_t free_blocks, llaisysTensor_t free_used,
+                                    llaisysTensor_t free_after);
+
+    /* New; no counterpart in the reference: the paged KV in 8 bits. Pools
+     * [num_blocks, nkvh, 16, 128] F8 hold e4m3 codes in a page format of their
+     * own (csrc/kernels/f8_page.hpp), k_scale and v_scale [num_blocks, nkvh] F32
+     * the scale 2^E of each block and kv head: E the least whole number, -100 at
+     * least, whose 448 * 2^E reaches the block's largest value. A value is read
+     * back within 2^-4 of its size, or within 2^-10 * 2^E where that is more.
+     * Block tables are as for the bf16 pool.
+     *
+     * Append: row r of k_new, v_new [T, nkvh, 128] BF16 to slots[r] (I64, block
+     * * 16 + offset, as llaisysPagedKVMap builds them; negative: the row is not
+     * written). A block's rows are one run: consecutive rows at consecutive
+     * slots. Rows that break it or begin a second one within 32 rows are not
+     * written (error bit 2); a block written from places of the batch further
+     * apart is the caller's mistake, and its contents are then undefined. A run
+     * that begins at a block's offset 0 starts the block's scale anew; otherwise
+     * the scale grows if the new rows need it, and the block's codes are
+     * re-encoded, which rounds only those that become subnormal. A value that is
+     * not finite is kept as NaN and leaves the scale alone. A slot past the
+     * pool: error bit 1. */
+    __export void llaisysPagedKVAppendF8(llaisysTensor_t k_pool, llaisysTensor_t v_pool, llaisysTensor_t k_scale,
+                                         llaisysTensor_t v_scale, llaisysTensor_t k_new, llaisysTensor_t v_new,
+                                         llaisysTensor_t slots);
+    /* llaisysPagedKVGather out of the 8-bit pool: k_out, v_out [T, nkvh, 128]
+     * BF16, which holds every value of the cache exactly. */
+    __export void llaisysPagedKVGatherF8(llaisysTensor_t k_out, llaisysTensor_t v_out, llaisysTensor_t k_pool,
+                                         llaisysTensor_t v_pool, llaisysTensor_t k_scale, llaisysTensor_t v_scale,
+                                         llaisysTensor_t block_table, llaisysTensor_t cu_seqlens);
+    /* llaisysPagedKVCopyBlocks of the 8-bit pool, scales included. */
+    __export void llaisysPagedKVCopyBlocksF8(llaisysTensor_t k_pool, llaisysTensor_t v_pool, llaisysTensor_t k_scale,
+                                             llaisysTensor_t v_scale, llaisysTensor_t pairs);
+    /* llaisysPagedAttention and llaisysPagedAttentionVarlen over the 8-bit pool:
+     * the same arguments otherwise, the softmax and the sums in 32 bits. */
+    __export void llaisysPagedAttentionF8(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool,
+                                          llaisysTensor_t v_pool, llaisysTensor_t k_scale, llaisysTensor_t v_scale,
+                                          llaisysTensor_t block_table, llaisysTensor_t ctx_len, float scale);
+    __export void llaisysPagedAttentionVarlenF8(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool,
+                                                llaisysTensor_t v_pool, llaisysTensor_t k_scale,
+                                                llaisysTensor_t v_scale, llaisysTensor_t block_table,
+                                                llaisysTensor_t cu_q, llaisysTensor_t ctx_len, float scale);
+
+    /* New; no counterpart in the reference. Rows of x [M, K] (F32, F16 or BF16)
+     * as 8-bit integers: scale[m] = max |x[m, :]| / 127 (F32 [M]) and q[m, k] =
+     * x[m, k] / scale[m] to the nearest whole number, ties to even (I8 [M, K]).
+     * A row of zeros has the scale 0; a row with a value that is not finite the
+     * scale NaN and codes 0. For activations (a scale per token) and, over a
+     * weight's rows, for its output channels. */
+    __export void llaisysQuantizeRows(llaisysTensor_t q, llaisysTensor_t scale, llaisysTensor_t x);
+    /* New; no counterpart in the reference (whose linear is ops.h:10).
+     * llaisysLinear in 8-bit integers: out[m, n] = (sum_k in[m, k] weight[n, k])
+     * * (in_scale[m] * weight_scale[n]) (+ bias[n], may be NULL), in [M, K] and
+     * weight [N, K] I8, scales F32, out and bias F32, F16 or BF16. The products
+     * are summed exactly in 32-bit integers (K <= 131071), the rest is 32-bit
+     * floats and one rounding. */
+    __export void llaisysLinearI8(llaisysTensor_t out, llaisysTensor_t in, llaisysTensor_t in_scale,
+                                  llaisysTensor_t weight, llaisysTensor_t weight_scale, llaisysTensor_t bias);
 }
 
 #endif /* LLAISYS_OPS_H */

@@ -62,7 +62,8 @@ __C {
 
     /* New (no reference counterpart): OR of the kernel-side error bits the
      * active AMD runtime has recorded (1 = block id outside the pool,
-     * 2 = context longer than the block table), clearing them. Synchronises
+     * 2 = context longer than the block table, 4 = embedding index outside the
+     * table, 8 = a free list with too few blocks), clearing them. Synchronises
      * the runtime's stream. 0 on CPU. */
     __export int llaisysGetDeviceErrorFlags(void);
 }

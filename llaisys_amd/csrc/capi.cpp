@@ -449,6 +449,87 @@ void llaisysPagedKVCopyBlocks(llaisysTensor_t k_pool, llaisysTensor_t v_pool, ll
     });
 }
 
+void llaisysPagedKVMap(llaisysTensor_t block_table, llaisysTensor_t cu_new, llaisysTensor_t ctx_after,
+                       llaisysTensor_t pos_ids, llaisysTensor_t slots, llaisysTensor_t ctx_len,
+                       llaisysTensor_t new_len, llaisysTensor_t free_blocks, llaisysTensor_t free_used,
+                       llaisysTensor_t free_after) {
+    guardedVoid([&] {
+        const char *w = "paged_kv_map";
+        llaisys::ops::pagedKVMap(unbox(block_table, w), unbox(cu_new, w), unbox(ctx_after, w), unbox(pos_ids, w),
+                                 unbox(slots, w), unbox(ctx_len, w), unbox(new_len, w), unboxOpt(free_blocks),
+                                 unboxOpt(free_used), unboxOpt(free_after));
+    });
+}
+
+void llaisysPagedKVAppendF8(llaisysTensor_t k_pool, llaisysTensor_t v_pool, llaisysTensor_t k_scale,
+                            llaisysTensor_t v_scale, llaisysTensor_t k_new, llaisysTensor_t v_new,
+                            llaisysTensor_t slots) {
+    guardedVoid([&] {
+        const char *w = "paged_kv_append_f8";
+        llaisys::ops::pagedKVAppendF8(unbox(k_pool, w), unbox(v_pool, w), unbox(k_scale, w), unbox(v_scale, w),
+                                      unbox(k_new, w), unbox(v_new, w), unbox(slots, w));
+    });
+}
+
+void llaisysPagedKVGatherF8(llaisysTensor_t k_out, llaisysTensor_t v_out, llaisysTensor_t k_pool,
+                            llaisysTensor_t v_pool, llaisysTensor_t k_scale, llaisysTensor_t v_scale,
+                            llaisysTensor_t block_table, llaisysTensor_t cu_seqlens) {
+    guardedVoid([&] {
+        const char *w = "paged_kv_gather_f8";
+        llaisys::ops::pagedKVGatherF8(unbox(k_out, w), unbox(v_out, w), unbox(k_pool, w), unbox(v_pool, w),
+                                      unbox(k_scale, w), unbox(v_scale, w), unbox(block_table, w),
+                                      unbox(cu_seqlens, w));
+    });
+}
+
+void llaisysPagedKVCopyBlocksF8(llaisysTensor_t k_pool, llaisysTensor_t v_pool, llaisysTensor_t k_scale,
+                                llaisysTensor_t v_scale, llaisysTensor_t pairs) {
+    guardedVoid([&] {
+        const char *w = "paged_kv_copy_blocks_f8";
+        llaisys::ops::pagedKVCopyBlocksF8(unbox(k_pool, w), unbox(v_pool, w), unbox(k_scale, w), unbox(v_scale, w),
+                                          unbox(pairs, w));
+    });
+}
+
+void llaisysPagedAttentionF8(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool, llaisysTensor_t v_pool,
+                             llaisysTensor_t k_scale, llaisysTensor_t v_scale, llaisysTensor_t block_table,
+                             llaisysTensor_t ctx_len, float scale) {
+    guardedVoid([&] {
+        const char *w = "paged_attention_f8";
+        llaisys::ops::pagedAttentionF8(unbox(out, w), unbox(q, w), unbox(k_pool, w), unbox(v_pool, w),
+                                       unbox(k_scale, w), unbox(v_scale, w), unbox(block_table, w),
+                                       unbox(ctx_len, w), nullptr, scale);
+    });
+}
+
+void llaisysPagedAttentionVarlenF8(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool,
+                                   llaisysTensor_t v_pool, llaisysTensor_t k_scale, llaisysTensor_t v_scale,
+                                   llaisysTensor_t block_table, llaisysTensor_t cu_q, llaisysTensor_t ctx_len,
+                                   float scale) {
+    guardedVoid([&] {
+        const char *w = "paged_attention_varlen_f8";
+        llaisys::ops::pagedAttentionF8(unbox(out, w), unbox(q, w), unbox(k_pool, w), unbox(v_pool, w),
+                                       unbox(k_scale, w), unbox(v_scale, w), unbox(block_table, w),
+                                       unbox(ctx_len, w), unbox(cu_q, w), scale);
+    });
+}
+
+void llaisysQuantizeRows(llaisysTensor_t q, llaisysTensor_t scale, llaisysTensor_t x) {
+    guardedVoid([&] {
+        const char *w = "quantize_rows";
+        llaisys::ops::quantizeRows(unbox(q, w), unbox(scale, w), unbox(x, w));
+    });
+}
+
+void llaisysLinearI8(llaisysTensor_t out, llaisysTensor_t in, llaisysTensor_t in_scale, llaisysTensor_t weight,
+                     llaisysTensor_t weight_scale, llaisysTensor_t bias) {
+    guardedVoid([&] {
+        const char *w = "linear_i8";
+        llaisys::ops::linearI8(unbox(out, w), unbox(in, w), unbox(in_scale, w), unbox(weight, w),
+                               unbox(weight_scale, w), unboxOpt(bias));
+    });
+}
+
 // ---------------- kv_cache.h
 namespace {
 llaisys::kvcache::BlockManager &mgr(llaisysKVBlockManager_t m) {

@@ -14,6 +14,8 @@ constexpr int kPageElems = kPageTokens * kHeadDim; // bf16 elements per (block, 
 
 enum class ElemType { F32, F16, BF16 };
 
+constexpr int kErrNoBlocks = 8; // error bit: a free list with too few blocks
+
 // Contiguous causal GQA attention (the reference's self_attention op).
 // Small grids (few query rows x heads) split the keys over workgroups into
 // fp32 partials in `workspace` (selfAttentionWorkspaceBytes; 0: none needed).
@@ -139,6 +141,47 @@ void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_
                   const int32_t *block_table, const int32_t *ctx_len, const int32_t *cu_q, int B, int T, int nh,
                   int nkvh, int max_pages, int num_blocks, float scale, const PagedAttentionPlan &plan,
                   float *records, int *err, int *queue, void *stream);
+
+// ---- a step's tables (paged_map.hip)
+// Per sequence its c = ctx_len and n = new_len: cu_new the prefix sums of n (at
+// most T), pages [ceil(c / 16), ceil((c + n) / 16)) of block_table from
+// free_blocks[*free_used ..) in the sequences' order, ctx_after = c + n,
+// *free_after; per row its position and its slot (block * 16 + offset; -1 and
+// position 0: none). free_blocks null: the pages are mapped already.
+// T, F < 2^30. ctx_after may be ctx_len, free_after free_used.
+void pagedMap(int32_t *block_table, int32_t *cu_new, int32_t *ctx_after, int64_t *pos_ids, int64_t *slots,
+              const int32_t *ctx_len, const int32_t *new_len, const int32_t *free_blocks, const int32_t *free_used,
+              int32_t *free_after, int B, int T, int max_pages, int F, int *err, void *stream);
+
+// ---- the 8-bit paged KV (paged_f8.hip; f8_page.hpp has the format)
+// Rows of k_new, v_new [T, nkvh, 128] bf16 into the pages at slots[T] (< 0:
+// not written). Consecutive slots of a block are consecutive rows; one run of
+// them writes a block.
+void pagedAppendF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const uint16_t *k_new,
+                   const uint16_t *v_new, const int64_t *slots, int T, int nkvh, int num_blocks, int *err,
+                   void *stream);
+void pagedGatherF8(uint16_t *k_out, uint16_t *v_out, const uint8_t *k_pool, const uint8_t *v_pool,
+                   const float *k_scale, const float *v_scale, const int32_t *block_table, const int32_t *cu_seqlens,
+                   int T, int B, int nkvh, int max_pages, int num_blocks, int *err, void *stream);
+void pagedCopyBlocksF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const int32_t *pairs, int P,
+                       int nkvh, int num_blocks, int *err, void *stream);
+// Attention over it, one query per sequence (cu_q null, T == B) or sequence b's
+// rows [cu_q[b], cu_q[b + 1]), causal.
+void pagedAttentionF8(void *out, bool out_f32, const uint16_t *q, const uint8_t *k_pool, const uint8_t *v_pool,
+                      const float *k_scale, const float *v_scale, const int32_t *block_table, const int32_t *ctx_len,
+                      const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
+                      int *err, void *stream);
+
+// ---- 8-bit integers (quant.hip)
+// scale[m] = max |x[m, :]| / 127 and q[m, k] = x[m, k] / scale[m] to the
+// nearest whole number (ties to even); a row with a value that is not finite
+// gets the scale NaN and zeros.
+void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K, void *stream);
+// y[M, N] = (xq . wq^T) * (xs[m] * ws[n]) (+ bias[n]), the products summed in
+// 32-bit integers (K <= kLinearI8MaxK), one rounding to t.
+constexpr int kLinearI8MaxK = 131071; // 128 * 128 * K < 2^31
+void linearI8(void *y, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const void *bias,
+              ElemType t, int M, int N, int K, void *stream);
 
 // ---- model ops (model_ops.hip, linear.cpp)
 constexpr int kMaxDims = 8;

@@ -74,6 +74,25 @@ void checkPool(const tensor_t &kp, const tensor_t &vp, const char *op) {
     LLAISYS_CHECK(kp->shape()[0] < size_t(1) << 31, op << ": too many blocks");
 }
 
+// The 8-bit pools: F8 of the same shape, with F32 scales [num_blocks, nkvh].
+void checkPoolF8(const tensor_t &kp, const tensor_t &vp, const tensor_t &ks, const tensor_t &vs, const char *op) {
+    for (auto *t : {&kp, &vp}) {
+        LLAISYS_CHECK((*t)->ndim() == 4 && (*t)->shape()[2] == size_t(K::kPageTokens) &&
+                          (*t)->shape()[3] == size_t(K::kHeadDim),
+                      op << ": pool must be [num_blocks, nkvh, 16, 128], got " << shapeStr(*t));
+        requireDtype(*t, LLAISYS_DTYPE_F8, op, "pool");
+        requireContiguous(*t, op, "pool");
+    }
+    LLAISYS_CHECK(kp->shape() == vp->shape(), op << ": K and V pools differ in shape");
+    LLAISYS_CHECK(kp->shape()[0] < size_t(1) << 31, op << ": too many blocks");
+    LLAISYS_CHECK(kp->shape()[1] <= 65535, op << ": too many kv heads");
+    for (auto *t : {&ks, &vs}) {
+        requireShape(*t, {kp->shape()[0], kp->shape()[1]}, op, "scale");
+        requireDtype(*t, LLAISYS_DTYPE_F32, op, "scale");
+        requireContiguous(*t, op, "scale");
+    }
+}
+
 void checkTable(const tensor_t &table, size_t B, const char *op) {
     LLAISYS_CHECK(table->ndim() == 2 && table->shape()[0] == B,
                   op << ": block_table must be [B=" << B << ", max_pages], got " << shapeStr(table));
@@ -262,11 +281,9 @@ namespace {
 struct AttnDims {
     size_t T, nh, nkvh, B;
 };
-AttnDims checkAttention(const char *op, const tensor_t &out, const tensor_t &q, const tensor_t &k_pool,
-                        const tensor_t &v_pool, const tensor_t &block_table, const tensor_t &ctx_len,
-                        const tensor_t &cu_q) {
-    LLAISYS_CHECK(out && q && k_pool && v_pool && block_table && ctx_len, op << ": null tensor");
-    checkPool(k_pool, v_pool, op);
+// The part that does not depend on the pools' type (checked before).
+AttnDims checkAttentionOver(const char *op, const tensor_t &out, const tensor_t &q, const tensor_t &k_pool,
+                            const tensor_t &block_table, const tensor_t &ctx_len, const tensor_t &cu_q) {
     const size_t nkvh = k_pool->shape()[1];
     LLAISYS_CHECK(q->ndim() == 3 && q->shape()[2] == size_t(K::kHeadDim),
                   op << ": q must be [T, nh, 128], got " << shapeStr(q));
@@ -289,6 +306,13 @@ AttnDims checkAttention(const char *op, const tensor_t &out, const tensor_t &q, 
         LLAISYS_CHECK(T == B, op << ": q must hold one query per sequence (T=" << T << ", B=" << B << ")");
     }
     return {T, nh, nkvh, B};
+}
+AttnDims checkAttention(const char *op, const tensor_t &out, const tensor_t &q, const tensor_t &k_pool,
+                        const tensor_t &v_pool, const tensor_t &block_table, const tensor_t &ctx_len,
+                        const tensor_t &cu_q) {
+    LLAISYS_CHECK(out && q && k_pool && v_pool && block_table && ctx_len, op << ": null tensor");
+    checkPool(k_pool, v_pool, op);
+    return checkAttentionOver(op, out, q, k_pool, block_table, ctx_len, cu_q);
 }
 
 } // namespace
@@ -380,6 +404,174 @@ void pagedAttentionNoAlloc(const tensor_t &out, const tensor_t &q, const tensor_
                           reinterpret_cast<const int32_t *>(block_table->data()),
                           reinterpret_cast<const int32_t *>(ctx_len->data()), int(B), int(nh), int(nkvh), max_pages,
                           int(k_pool->shape()[0]), scale, errWord(), streamOf());
+}
+
+void pagedKVMap(const tensor_t &block_table, const tensor_t &cu_new, const tensor_t &ctx_after, const tensor_t &pos_ids,
+                const tensor_t &slots, const tensor_t &ctx_len, const tensor_t &new_len, const tensor_t &free_blocks,
+                const tensor_t &free_used, const tensor_t &free_after) {
+    const char *op = "paged_kv_map";
+    LLAISYS_CHECK(block_table && cu_new && ctx_after && pos_ids && slots && ctx_len && new_len, op << ": null tensor");
+    LLAISYS_CHECK(!free_blocks == !free_used && !free_blocks == !free_after,
+                  op << ": free_blocks, free_used and free_after go together");
+    const size_t B = ctx_len->ndim() == 1 ? ctx_len->shape()[0] : 0;
+    checkI32Vec(ctx_len, B, op, "ctx_len");
+    checkI32Vec(new_len, B, op, "new_len");
+    checkI32Vec(ctx_after, B, op, "ctx_after");
+    checkI32Vec(cu_new, B + 1, op, "cu_new");
+    checkTable(block_table, B, op);
+    for (const auto *t : {&slots, &pos_ids}) {
+        const char *name = t == &slots ? "slots" : "pos_ids";
+        LLAISYS_CHECK((*t)->ndim() == 1 && (*t)->shape() == slots->shape(),
+                      op << ": slots and pos_ids must be [T], got " << shapeStr(*t));
+        requireDtype(*t, LLAISYS_DTYPE_I64, op, name);
+        requireContiguous(*t, op, name);
+    }
+    const size_t T = slots->shape()[0], max_pages = block_table->shape()[1];
+    size_t F = 0;
+    if (free_blocks) {
+        F = free_blocks->ndim() == 1 ? free_blocks->shape()[0] : 0;
+        checkI32Vec(free_blocks, F, op, "free_blocks");
+        checkI32Vec(free_used, 1, op, "free_used");
+        checkI32Vec(free_after, 1, op, "free_after");
+    }
+    constexpr size_t kMost = size_t(1) << 30; // the sums' cap
+    LLAISYS_CHECK(T < kMost - 1 && F < kMost - 1 && B < kMost && max_pages < kMost,
+                  op << ": sizes must be under 2^30");
+    const bool host = onHost(op, {&block_table, &cu_new, &ctx_after, &pos_ids, &slots, &ctx_len, &new_len,
+                                  &free_blocks, &free_used, &free_after});
+    auto i32 = [](const tensor_t &t) { return t ? reinterpret_cast<int32_t *>(t->data()) : nullptr; };
+    auto i64 = [](const tensor_t &t) { return reinterpret_cast<int64_t *>(t->data()); };
+    if (host)
+        C::pagedMap(i32(block_table), i32(cu_new), i32(ctx_after), i64(pos_ids), i64(slots), i32(ctx_len),
+                    i32(new_len), i32(free_blocks), i32(free_used), i32(free_after), int(B), int(T), int(max_pages),
+                    int(F), errWord());
+    else
+        K::pagedMap(i32(block_table), i32(cu_new), i32(ctx_after), i64(pos_ids), i64(slots), i32(ctx_len),
+                    i32(new_len), i32(free_blocks), i32(free_used), i32(free_after), int(B), int(T), int(max_pages),
+                    int(F), errWord(), streamOf());
+}
+
+void pagedKVAppendF8(const tensor_t &k_pool, const tensor_t &v_pool, const tensor_t &k_scale, const tensor_t &v_scale,
+                     const tensor_t &k_new, const tensor_t &v_new, const tensor_t &slots) {
+    const char *op = "paged_kv_append_f8";
+    LLAISYS_CHECK(k_pool && v_pool && k_scale && v_scale && k_new && v_new && slots, op << ": null tensor");
+    checkPoolF8(k_pool, v_pool, k_scale, v_scale, op);
+    const size_t nkvh = k_pool->shape()[1];
+    LLAISYS_CHECK(k_new->ndim() == 3 && k_new->shape()[1] == nkvh && k_new->shape()[2] == size_t(K::kHeadDim),
+                  op << ": k_new must be [T, nkvh=" << nkvh << ", 128], got " << shapeStr(k_new));
+    LLAISYS_CHECK(v_new->shape() == k_new->shape(), op << ": v_new shape differs from k_new");
+    for (const auto *t : {&k_new, &v_new}) {
+        requireDtype(*t, LLAISYS_DTYPE_BF16, op, "k_new and v_new");
+        requireContiguous(*t, op, "k_new and v_new");
+    }
+    const size_t T = k_new->shape()[0];
+    requireShape(slots, {T}, op, "slots");
+    requireDtype(slots, LLAISYS_DTYPE_I64, op, "slots");
+    requireContiguous(slots, op, "slots");
+    LLAISYS_CHECK(T < size_t(1) << 31, op << ": too many rows");
+    const bool host = onHost(op, {&k_pool, &v_pool, &k_scale, &v_scale, &k_new, &v_new, &slots});
+    if (T == 0 || nkvh == 0) return;
+    auto *kp = reinterpret_cast<uint8_t *>(k_pool->data());
+    auto *vp = reinterpret_cast<uint8_t *>(v_pool->data());
+    auto *ks = reinterpret_cast<float *>(k_scale->data());
+    auto *vs = reinterpret_cast<float *>(v_scale->data());
+    const auto *kn = reinterpret_cast<const uint16_t *>(k_new->data());
+    const auto *vn = reinterpret_cast<const uint16_t *>(v_new->data());
+    const auto *sl = reinterpret_cast<const int64_t *>(slots->data());
+    const int nb = int(k_pool->shape()[0]);
+    if (host)
+        C::pagedAppendF8(kp, vp, ks, vs, kn, vn, sl, int(T), int(nkvh), nb, errWord());
+    else
+        K::pagedAppendF8(kp, vp, ks, vs, kn, vn, sl, int(T), int(nkvh), nb, errWord(), streamOf());
+}
+
+void pagedKVGatherF8(const tensor_t &k_out, const tensor_t &v_out, const tensor_t &k_pool, const tensor_t &v_pool,
+                     const tensor_t &k_scale, const tensor_t &v_scale, const tensor_t &block_table,
+                     const tensor_t &cu_seqlens) {
+    const char *op = "paged_kv_gather_f8";
+    LLAISYS_CHECK(k_out && v_out && k_pool && v_pool && k_scale && v_scale && block_table && cu_seqlens,
+                  op << ": null tensor");
+    checkPoolF8(k_pool, v_pool, k_scale, v_scale, op);
+    const size_t nkvh = k_pool->shape()[1];
+    LLAISYS_CHECK(k_out->ndim() == 3 && k_out->shape()[1] == nkvh && k_out->shape()[2] == size_t(K::kHeadDim),
+                  op << ": k_out must be [T, nkvh=" << nkvh << ", 128], got " << shapeStr(k_out));
+    LLAISYS_CHECK(v_out->shape() == k_out->shape(), op << ": v_out shape differs from k_out");
+    for (const auto *t : {&k_out, &v_out}) {
+        requireDtype(*t, LLAISYS_DTYPE_BF16, op, "k_out and v_out");
+        requireContiguous(*t, op, "k_out and v_out");
+    }
+    LLAISYS_CHECK(cu_seqlens->ndim() == 1 && cu_seqlens->shape()[0] >= 1, op << ": cu_seqlens must be [B+1]");
+    const size_t B = cu_seqlens->shape()[0] - 1;
+    checkI32Vec(cu_seqlens, B + 1, op, "cu_seqlens");
+    checkTable(block_table, B, op);
+    LLAISYS_CHECK(B <= 65535, op << ": at most 65535 sequences");
+    LLAISYS_CHECK(k_out->shape()[0] < size_t(1) << 31 && block_table->shape()[1] < size_t(1) << 27,
+                  op << ": too many rows or pages");
+    const bool host = onHost(op, {&k_out, &v_out, &k_pool, &v_pool, &k_scale, &v_scale, &block_table, &cu_seqlens});
+    auto *ko = reinterpret_cast<uint16_t *>(k_out->data());
+    auto *vo = reinterpret_cast<uint16_t *>(v_out->data());
+    const auto *kp = reinterpret_cast<const uint8_t *>(k_pool->data());
+    const auto *vp = reinterpret_cast<const uint8_t *>(v_pool->data());
+    const auto *ks = reinterpret_cast<const float *>(k_scale->data());
+    const auto *vs = reinterpret_cast<const float *>(v_scale->data());
+    const auto *tab = reinterpret_cast<const int32_t *>(block_table->data());
+    const auto *cu = reinterpret_cast<const int32_t *>(cu_seqlens->data());
+    const int T = int(k_out->shape()[0]), maxp = int(block_table->shape()[1]), nb = int(k_pool->shape()[0]);
+    if (nkvh == 0) return;
+    if (host)
+        C::pagedGatherF8(ko, vo, kp, vp, ks, vs, tab, cu, T, int(B), int(nkvh), maxp, nb, errWord());
+    else
+        K::pagedGatherF8(ko, vo, kp, vp, ks, vs, tab, cu, T, int(B), int(nkvh), maxp, nb, errWord(), streamOf());
+}
+
+void pagedKVCopyBlocksF8(const tensor_t &k_pool, const tensor_t &v_pool, const tensor_t &k_scale,
+                         const tensor_t &v_scale, const tensor_t &pairs) {
+    const char *op = "paged_kv_copy_blocks_f8";
+    LLAISYS_CHECK(k_pool && v_pool && k_scale && v_scale && pairs, op << ": null tensor");
+    checkPoolF8(k_pool, v_pool, k_scale, v_scale, op);
+    LLAISYS_CHECK(pairs->ndim() == 2 && pairs->shape()[1] == 2, op << ": pairs must be [P, 2], got " << shapeStr(pairs));
+    requireDtype(pairs, LLAISYS_DTYPE_I32, op, "pairs");
+    requireContiguous(pairs, op, "pairs");
+    LLAISYS_CHECK(pairs->shape()[0] < size_t(1) << 31, op << ": too many pairs");
+    const bool host = onHost(op, {&k_pool, &v_pool, &k_scale, &v_scale, &pairs});
+    auto *kp = reinterpret_cast<uint8_t *>(k_pool->data());
+    auto *vp = reinterpret_cast<uint8_t *>(v_pool->data());
+    auto *ks = reinterpret_cast<float *>(k_scale->data());
+    auto *vs = reinterpret_cast<float *>(v_scale->data());
+    const auto *pr = reinterpret_cast<const int32_t *>(pairs->data());
+    const int P = int(pairs->shape()[0]), nkvh = int(k_pool->shape()[1]), nb = int(k_pool->shape()[0]);
+    if (host)
+        C::pagedCopyBlocksF8(kp, vp, ks, vs, pr, P, nkvh, nb, errWord());
+    else
+        K::pagedCopyBlocksF8(kp, vp, ks, vs, pr, P, nkvh, nb, errWord(), streamOf());
+}
+
+void pagedAttentionF8(const tensor_t &out, const tensor_t &q, const tensor_t &k_pool, const tensor_t &v_pool,
+                      const tensor_t &k_scale, const tensor_t &v_scale, const tensor_t &block_table,
+                      const tensor_t &ctx_len, const tensor_t &cu_q, float scale) {
+    const char *op = cu_q ? "paged_attention_varlen_f8" : "paged_attention_f8";
+    LLAISYS_CHECK(out && q && k_pool && v_pool && k_scale && v_scale && block_table && ctx_len, op << ": null tensor");
+    checkPoolF8(k_pool, v_pool, k_scale, v_scale, op);
+    const auto [T, nh, nkvh, B] = checkAttentionOver(op, out, q, k_pool, block_table, ctx_len, cu_q);
+    const bool host = onHost(op, {&out, &q, &k_pool, &v_pool, &k_scale, &v_scale, &block_table, &ctx_len, &cu_q});
+    if (T == 0 || B == 0) return;
+    const int max_pages = int(block_table->shape()[1]);
+    LLAISYS_CHECK(max_pages > 0, op << ": block_table has no pages");
+    const bool f32 = out->dtype() == LLAISYS_DTYPE_F32;
+    const auto *qp = reinterpret_cast<const uint16_t *>(q->data());
+    const auto *kp = reinterpret_cast<const uint8_t *>(k_pool->data());
+    const auto *vp = reinterpret_cast<const uint8_t *>(v_pool->data());
+    const auto *ks = reinterpret_cast<const float *>(k_scale->data());
+    const auto *vs = reinterpret_cast<const float *>(v_scale->data());
+    const auto *tab = reinterpret_cast<const int32_t *>(block_table->data());
+    const auto *ctx = reinterpret_cast<const int32_t *>(ctx_len->data());
+    const auto *cu = cu_q ? reinterpret_cast<const int32_t *>(cu_q->data()) : nullptr;
+    const int nb = int(k_pool->shape()[0]);
+    if (host)
+        return C::pagedAttentionF8(out->data(), f32, qp, kp, vp, ks, vs, tab, ctx, cu, int(B), int(T), int(nh),
+                                   int(nkvh), max_pages, nb, scale, errWord());
+    K::pagedAttentionF8(out->data(), f32, qp, kp, vp, ks, vs, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh),
+                        max_pages, nb, scale, errWord(), streamOf());
 }
 
 } // namespace llaisys::ops

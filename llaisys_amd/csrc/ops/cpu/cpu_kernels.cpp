@@ -4,6 +4,7 @@
 #include "cpu_kernels.hpp"
 
 #include "../../common.hpp"
+#include "../../kernels/f8_page.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -577,9 +578,14 @@ void pagedCopyBlocks(uint16_t *k_pool, uint16_t *v_pool, const int32_t *pairs, i
     }
 }
 
-void pagedAttention(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
-                    const int32_t *table, const int32_t *ctx, const int32_t *cu_q, int B, int T, int nh, int nkvh,
-                    int max_pages, int num_blocks, float scale, int *err) {
+namespace {
+
+// Paged attention over pages that read(K rows, V rows, unit, n) widens: the
+// first n tokens of (block, kv head) page `unit`, 128 floats each.
+template <typename Read>
+void attendPages(void *out, bool out_f32, const uint16_t *q, const int32_t *table, const int32_t *ctx,
+                 const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
+                 int *err, Read &&read) {
     const int G = nh / nkvh;
     auto store = [&](size_t row, int h, const float *o) {
         const size_t base = (row * nh + h) * kHeadDim;
@@ -620,13 +626,7 @@ void pagedAttention(void *out, bool out_f32, const uint16_t *q, const uint16_t *
                 std::fill(skip.begin() + 16 * p, skip.begin() + 16 * p + n, 1);
                 continue;
             }
-            const uint16_t *kp = k_pool + (size_t(blk) * nkvh + hk) * kPageElems;
-            const uint16_t *vp = v_pool + (size_t(blk) * nkvh + hk) * kPageElems;
-            for (int t = 0; t < n; ++t)
-                for (int dd = 0; dd < kHeadDim; ++dd) {
-                    K[size_t(16 * p + t) * kHeadDim + dd] = bf16ToF32(kp[kIndex(t, dd)]);
-                    V[size_t(16 * p + t) * kHeadDim + dd] = bf16ToF32(vp[vIndex(t, dd)]);
-                }
+            read(K.data() + size_t(16 * p) * kHeadDim, V.data() + size_t(16 * p) * kHeadDim, size_t(blk) * nkvh + hk, n);
         }
         float qf[kHeadDim], o[kHeadDim];
         for (int i = 0; i < Lq; ++i) {
@@ -641,6 +641,259 @@ void pagedAttention(void *out, bool out_f32, const uint16_t *q, const uint16_t *
             }
         }
     });
+}
+
+} // namespace
+
+void pagedAttention(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
+                    const int32_t *table, const int32_t *ctx, const int32_t *cu_q, int B, int T, int nh, int nkvh,
+                    int max_pages, int num_blocks, float scale, int *err) {
+    attendPages(out, out_f32, q, table, ctx, cu_q, B, T, nh, nkvh, max_pages, num_blocks, scale, err,
+                [&](float *K, float *V, size_t unit, int n) {
+                    const uint16_t *kp = k_pool + unit * kPageElems, *vp = v_pool + unit * kPageElems;
+                    for (int t = 0; t < n; ++t)
+                        for (int dd = 0; dd < kHeadDim; ++dd) {
+                            K[size_t(t) * kHeadDim + dd] = bf16ToF32(kp[kIndex(t, dd)]);
+                            V[size_t(t) * kHeadDim + dd] = bf16ToF32(vp[vIndex(t, dd)]);
+                        }
+                });
+}
+
+void pagedMap(int32_t *table, int32_t *cu, int32_t *after, int64_t *pos, int64_t *slots, const int32_t *ctx,
+              const int32_t *fresh, const int32_t *free_blocks, const int32_t *free_used, int32_t *free_after, int B,
+              int T, int max_pages, int F, int *err) {
+    const int used = free_blocks ? *free_used : 0;
+    const int64_t avail = free_blocks && used >= 0 ? std::max<int64_t>(0, int64_t(F) - used) : 0;
+    int64_t rows = 0, wanted = 0, taken = 0; // rows so far; blocks asked for; blocks of those that fit
+    cu[0] = 0;
+    for (int b = 0; b < B; ++b) {
+        const int64_t c = ctx[b], n = fresh[b], asked = std::max<int64_t>(n, 0);
+        const int64_t begin = std::min<int64_t>(rows, T), end = std::min<int64_t>(rows + asked, T);
+        rows += asked;
+        int32_t *row = table + size_t(b) * max_pages;
+        bool ok = c >= 0 && n >= 0 && c + n <= int64_t(max_pages) * kPageTokens && rows <= T;
+        if (!ok) raiseFlag(err, kErrTooLong);
+        if (ok && n > 0 && (c % kPageTokens != 0 || !free_blocks) && row[c / kPageTokens] < 0) {
+            raiseFlag(err, kErrBadBlock);
+            ok = false;
+        }
+        if (ok && free_blocks) {
+            const int64_t first = (c + kPageTokens - 1) / kPageTokens, last = (c + n + kPageTokens - 1) / kPageTokens;
+            wanted += last - first;
+            if (last > first && wanted > avail) {
+                raiseFlag(err, kernels::kErrNoBlocks);
+                ok = false;
+            } else if (last > first) {
+                for (int64_t p = first; p < last; ++p) row[p] = free_blocks[used + taken + p - first];
+                taken = wanted;
+            }
+        }
+        bool put = ok && n > 0; // a sequence whose first row has no block gets no slot at all
+        for (int64_t r = begin; r < end; ++r) {
+            const int64_t p = c + r - begin;
+            int32_t id = -1;
+            if (put) {
+                id = row[p / kPageTokens];
+                if (id < 0) raiseFlag(err, kErrBadBlock);
+                if (r == begin) put = id >= 0;
+            }
+            pos[r] = id >= 0 ? p : 0;
+            slots[r] = id >= 0 ? int64_t(id) * kPageTokens + p % kPageTokens : -1;
+        }
+        cu[b + 1] = int32_t(end);
+        after[b] = int32_t(c + (ok ? n : 0));
+    }
+    for (int64_t r = rows; r < T; ++r) {
+        pos[r] = 0;
+        slots[r] = -1;
+    }
+    if (free_blocks) *free_after = int32_t(used + taken);
+}
+
+namespace {
+
+// |y| <= 448, or not finite (the code of NaN); to the nearest code, ties to even.
+uint8_t f32ToE4m3(float y) {
+    uint32_t u;
+    std::memcpy(&u, &y, 4);
+    const uint32_t sign = (u >> 24) & 0x80u, a = u & 0x7fffffffu;
+    if (a >= 0x7f800000u) return uint8_t(sign | 0x7fu);
+    if (a < 0x3c800000u) // under 2^-6: subnormal, steps of 2^-9
+        return uint8_t(sign | uint32_t(std::nearbyint(std::fabs(y) * 512.f)));
+    return uint8_t(sign | (((a + 0x7ffffu + ((a >> 20) & 1u)) >> 20) - (120u << 3)));
+}
+
+float e4m3ToF32(uint8_t c) {
+    const int e = (c >> 3) & 15, m = c & 7;
+    float v = e == 15 && m == 7 ? std::numeric_limits<float>::quiet_NaN()
+              : e               ? std::ldexp(float(8 + m), e - 10)
+                                : std::ldexp(float(m), -9);
+    return c & 0x80 ? -v : v;
+}
+
+// One pool's part of pagedAppendF8: n rows of kv head h from `rows` on into
+// slots off.. of a block.
+void appendRun(uint8_t *page, float *scale, const uint16_t *rows, size_t stride, int off, int n, bool is_v) {
+    using namespace kernels;
+    int top = 0;
+    for (int t = 0; t < n; ++t)
+        for (int d = 0; d < kHeadDim; ++d) {
+            const int a = rows[t * stride + d] & 0x7fff;
+            if (a < 0x7f80) top = std::max(top, a);
+        }
+    const int was = off == 0 ? kF8LeastExp : f8ExpOfScale(*scale), now = std::max(was, f8ExpOf(top));
+    if (off != 0 && now != was)
+        for (int i = 0; i < kF8PageBytes; ++i) page[i] = f32ToE4m3(std::ldexp(e4m3ToF32(page[i]), was - now));
+    for (int t = 0; t < n; ++t)
+        for (int d = 0; d < kHeadDim; ++d)
+            page[is_v ? vF8Index(off + t, d) : kF8Index(off + t, d)] =
+                f32ToE4m3(std::ldexp(bf16ToF32(rows[t * stride + d]), -now));
+    *scale = f8Exp2(now);
+}
+
+// The first n tokens of a page as floats.
+void readF8(float *K, float *V, const uint8_t *kp, const uint8_t *vp, float ks, float vs, int n) {
+    using namespace kernels;
+    ks = f8Exp2(f8ExpOfScale(ks));
+    vs = f8Exp2(f8ExpOfScale(vs));
+    for (int t = 0; t < n; ++t)
+        for (int d = 0; d < kHeadDim; ++d) {
+            K[size_t(t) * kHeadDim + d] = e4m3ToF32(kp[kF8Index(t, d)]) * ks;
+            V[size_t(t) * kHeadDim + d] = e4m3ToF32(vp[vF8Index(t, d)]) * vs;
+        }
+}
+
+} // namespace
+
+void pagedAppendF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const uint16_t *k_new,
+                   const uint16_t *v_new, const int64_t *slots, int T, int nkvh, int num_blocks, int *err) {
+    parallelFor(size_t(T), 64, [&](size_t r) {
+        const int64_t slot = slots[r];
+        if (slot < 0) return;
+        const int64_t block = slot / kPageTokens;
+        if (block >= num_blocks) {
+            raiseFlag(err, kErrBadBlock);
+            return;
+        }
+        for (size_t back = 1; back <= size_t(kernels::kF8LookBack) && back <= r; ++back) {
+            if (slots[r - back] < 0 || slots[r - back] / kPageTokens != block) continue;
+            if (slots[r - 1] + 1 != slot) raiseFlag(err, kErrTooLong);
+            return; // within a run that began earlier, or a second run of the block
+        }
+        const int off = int(slot % kPageTokens);
+        int n = 1;
+        while (off + n < kPageTokens && r + n < size_t(T) && slots[r + n] == slot + n) ++n;
+        for (int h = 0; h < nkvh; ++h) {
+            const size_t unit = size_t(block) * nkvh + h, row = (r * nkvh + h) * kHeadDim;
+            appendRun(k_pool + unit * kernels::kF8PageBytes, k_scale + unit, k_new + row, size_t(nkvh) * kHeadDim, off, n, false);
+            appendRun(v_pool + unit * kernels::kF8PageBytes, v_scale + unit, v_new + row, size_t(nkvh) * kHeadDim, off, n, true);
+        }
+    });
+}
+
+void pagedGatherF8(uint16_t *k_out, uint16_t *v_out, const uint8_t *k_pool, const uint8_t *v_pool,
+                   const float *k_scale, const float *v_scale, const int32_t *table, const int32_t *cu, int T, int B,
+                   int nkvh, int max_pages, int num_blocks, int *err) {
+    parallelFor(size_t(B), 1, [&](size_t b) {
+        const int row0 = cu[b], len = cu[b + 1] - row0;
+        if (len <= 0) return;
+        if (row0 < 0 || cu[b + 1] > T) {
+            raiseFlag(err, kErrTooLong);
+            return;
+        }
+        if (len > max_pages * kPageTokens) raiseFlag(err, kErrTooLong);
+        float K[kPageElems], V[kPageElems];
+        for (int p = 0; p < std::min((len + 15) / 16, max_pages); ++p) {
+            const int blk = table[b * size_t(max_pages) + p];
+            if (blk < 0 || blk >= num_blocks) {
+                raiseFlag(err, kErrBadBlock);
+                continue;
+            }
+            const int n = std::min(16, len - 16 * p);
+            for (int h = 0; h < nkvh; ++h) {
+                const size_t unit = size_t(blk) * nkvh + h;
+                readF8(K, V, k_pool + unit * kernels::kF8PageBytes, v_pool + unit * kernels::kF8PageBytes,
+                       k_scale[unit], v_scale[unit], n);
+                for (int t = 0; t < n; ++t)
+                    for (int d = 0; d < kHeadDim; ++d) {
+                        const size_t at = (size_t(row0 + 16 * p + t) * nkvh + h) * kHeadDim + d;
+                        k_out[at] = f32ToBf16(K[t * kHeadDim + d]);
+                        v_out[at] = f32ToBf16(V[t * kHeadDim + d]);
+                    }
+            }
+        }
+    });
+}
+
+void pagedCopyBlocksF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const int32_t *pairs, int P,
+                       int nkvh, int num_blocks, int *err) {
+    const size_t per_block = size_t(nkvh) * kernels::kF8PageBytes;
+    for (int i = 0; i < P; ++i) { // in order: a later pair may read a block an earlier one wrote
+        const int s = pairs[2 * i], d = pairs[2 * i + 1];
+        if (s < 0 || s >= num_blocks || d < 0 || d >= num_blocks) {
+            raiseFlag(err, kErrBadBlock);
+            continue;
+        }
+        std::memmove(k_pool + d * per_block, k_pool + s * per_block, per_block);
+        std::memmove(v_pool + d * per_block, v_pool + s * per_block, per_block);
+        std::memmove(k_scale + size_t(d) * nkvh, k_scale + size_t(s) * nkvh, nkvh * sizeof(float));
+        std::memmove(v_scale + size_t(d) * nkvh, v_scale + size_t(s) * nkvh, nkvh * sizeof(float));
+    }
+}
+
+void pagedAttentionF8(void *out, bool out_f32, const uint16_t *q, const uint8_t *k_pool, const uint8_t *v_pool,
+                      const float *k_scale, const float *v_scale, const int32_t *table, const int32_t *ctx,
+                      const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
+                      int *err) {
+    attendPages(out, out_f32, q, table, ctx, cu_q, B, T, nh, nkvh, max_pages, num_blocks, scale, err,
+                [&](float *K, float *V, size_t unit, int n) {
+                    readF8(K, V, k_pool + unit * kernels::kF8PageBytes, v_pool + unit * kernels::kF8PageBytes,
+                           k_scale[unit], v_scale[unit], n);
+                });
+}
+
+template <typename T> struct QuantizeOp {
+    static void run(int8_t *q, float *scale, const void *x, int M, int K) {
+        parallelFor(size_t(M), 4, [&](size_t m) {
+            float top = 0.f;
+            bool finite = true;
+            for (int k = 0; k < K; ++k) {
+                const float v = std::fabs(Elem<T>::ld(x, m * K + k));
+                finite = finite && std::isfinite(v);
+                top = std::max(top, v);
+            }
+            const float s = finite ? top / 127.f : std::numeric_limits<float>::quiet_NaN();
+            scale[m] = s;
+            // (the 64-bit quotient of two 32-bit numbers is a tie only where the exact one is)
+            for (int k = 0; k < K; ++k)
+                q[m * K + k] = s > 0.f ? int8_t(std::max(-127.0, std::min(127.0, std::nearbyint(
+                                             double(Elem<T>::ld(x, m * K + k)) / double(s)))))
+                                       : int8_t(0);
+        });
+    }
+};
+
+void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K) {
+    byType<QuantizeOp>(t, q, scale, x, M, K);
+}
+
+template <typename T> struct LinearI8Op {
+    static void run(void *y, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const void *bias,
+                    int M, int N, int K) {
+        parallelFor(size_t(M) * N, 64, [&](size_t i) {
+            const size_t m = i / N, n = i % N;
+            int32_t sum = 0;
+            for (int k = 0; k < K; ++k) sum += int32_t(xq[m * K + k]) * int32_t(wq[n * K + k]);
+            float v = float(sum) * (xs[m] * ws[n]);
+            if (bias) v += Elem<T>::ld(bias, n);
+            Elem<T>::st(y, i, v);
+        });
+    }
+};
+
+void linearI8(void *y, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const void *bias,
+              ElemType t, int M, int N, int K) {
+    byType<LinearI8Op>(t, y, xq, xs, wq, ws, bias, M, N, K);
 }
 
 } // namespace llaisys::cpu

@@ -59,4 +59,26 @@ void pagedAttention(void *out, bool out_f32, const uint16_t *q, const uint16_t *
                     const int32_t *table, const int32_t *ctx, const int32_t *cu_q, int B, int T, int nh, int nkvh,
                     int max_pages, int num_blocks, float scale, int *err);
 
+// A step's tables, as kernels::pagedMap.
+void pagedMap(int32_t *table, int32_t *cu, int32_t *after, int64_t *pos, int64_t *slots, const int32_t *ctx,
+              const int32_t *fresh, const int32_t *free_blocks, const int32_t *free_used, int32_t *free_after, int B,
+              int T, int max_pages, int F, int *err);
+// The 8-bit paged KV (kernels/f8_page.hpp has the format): the same codes and
+// scales as the device kernels write.
+void pagedAppendF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const uint16_t *k_new,
+                   const uint16_t *v_new, const int64_t *slots, int T, int nkvh, int num_blocks, int *err);
+void pagedGatherF8(uint16_t *k_out, uint16_t *v_out, const uint8_t *k_pool, const uint8_t *v_pool,
+                   const float *k_scale, const float *v_scale, const int32_t *table, const int32_t *cu, int T, int B,
+                   int nkvh, int max_pages, int num_blocks, int *err);
+void pagedCopyBlocksF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const int32_t *pairs, int P,
+                       int nkvh, int num_blocks, int *err);
+void pagedAttentionF8(void *out, bool out_f32, const uint16_t *q, const uint8_t *k_pool, const uint8_t *v_pool,
+                      const float *k_scale, const float *v_scale, const int32_t *table, const int32_t *ctx,
+                      const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
+                      int *err);
+// 8-bit integers: rows to codes with a scale each, and the product.
+void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K);
+void linearI8(void *y, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const void *bias,
+              ElemType t, int M, int N, int K);
+
 } // namespace llaisys::cpu

@@ -178,6 +178,55 @@ void linearPacked(const tensor_t &out, const tensor_t &in, const tensor_t &packe
     }
 }
 
+void quantizeRows(const tensor_t &q, const tensor_t &scale, const tensor_t &x) {
+    const char *op = "quantize_rows";
+    LLAISYS_CHECK(q && scale && x, op << ": null tensor");
+    LLAISYS_CHECK(x->ndim() == 2 && q->shape() == x->shape(), op << ": q and x must be [M, K], got " << shapeOf(q)
+                                                                 << " and " << shapeOf(x));
+    const size_t M = x->shape()[0], Kd = x->shape()[1];
+    LLAISYS_CHECK(scale->ndim() == 1 && scale->shape()[0] == M, op << ": scale must be [" << M << "]");
+    LLAISYS_CHECK(q->dtype() == LLAISYS_DTYPE_I8 && scale->dtype() == LLAISYS_DTYPE_F32,
+                  op << ": q must be i8 and scale f32");
+    LLAISYS_CHECK(M < size_t(1) << 31 && Kd < size_t(1) << 31, op << ": sizes must be under 2^31");
+    const auto t = floatType(x, op);
+    const bool host = onHost(op, {&q, &scale, &x});
+    auto *qp = reinterpret_cast<int8_t *>(q->data());
+    auto *sp = reinterpret_cast<float *>(scale->data());
+    if (host) return C::quantizeRows(qp, sp, x->data(), t, int(M), int(Kd));
+    K::quantizeRows(qp, sp, x->data(), t, int(M), int(Kd), stream());
+}
+
+void linearI8(const tensor_t &out, const tensor_t &in, const tensor_t &in_scale, const tensor_t &weight,
+              const tensor_t &weight_scale, const tensor_t &bias) {
+    const char *op = "linear_i8";
+    LLAISYS_CHECK(out && in && in_scale && weight && weight_scale, op << ": null tensor");
+    LLAISYS_CHECK(in->ndim() == 2 && weight->ndim() == 2 && out->ndim() == 2, op << ": in, weight, out must be 2-D");
+    const size_t M = in->shape()[0], Kd = in->shape()[1], N = weight->shape()[0];
+    LLAISYS_CHECK(weight->shape()[1] == Kd, op << ": weight " << shapeOf(weight) << " does not match in " << shapeOf(in));
+    LLAISYS_CHECK(out->shape()[0] == M && out->shape()[1] == N, op << ": out must be [" << M << ", " << N << "]");
+    LLAISYS_CHECK(in_scale->ndim() == 1 && in_scale->shape()[0] == M, op << ": in_scale must be [" << M << "]");
+    LLAISYS_CHECK(weight_scale->ndim() == 1 && weight_scale->shape()[0] == N,
+                  op << ": weight_scale must be [" << N << "]");
+    if (bias) LLAISYS_CHECK(bias->ndim() == 1 && bias->shape()[0] == N, op << ": bias must be [" << N << "]");
+    LLAISYS_CHECK(in->dtype() == LLAISYS_DTYPE_I8 && weight->dtype() == LLAISYS_DTYPE_I8,
+                  op << ": in and weight must be i8");
+    LLAISYS_CHECK(in_scale->dtype() == LLAISYS_DTYPE_F32 && weight_scale->dtype() == LLAISYS_DTYPE_F32,
+                  op << ": scales must be f32");
+    sameDtype(op, {&out, &bias});
+    LLAISYS_CHECK(Kd <= size_t(K::kLinearI8MaxK), op << ": K is at most " << K::kLinearI8MaxK
+                                                     << " (32-bit sums), got " << Kd);
+    LLAISYS_CHECK(M < size_t(1) << 31 && N < size_t(1) << 31 && M * N < size_t(1) << 38, op << ": out is too large");
+    const auto t = floatType(out, op);
+    const bool host = onHost(op, {&out, &in, &in_scale, &weight, &weight_scale, &bias});
+    const auto *xq = reinterpret_cast<const int8_t *>(in->data());
+    const auto *xs = reinterpret_cast<const float *>(in_scale->data());
+    const auto *wq = reinterpret_cast<const int8_t *>(weight->data());
+    const auto *ws = reinterpret_cast<const float *>(weight_scale->data());
+    if (host)
+        return C::linearI8(out->data(), xq, xs, wq, ws, bias ? bias->data() : nullptr, t, int(M), int(N), int(Kd));
+    K::linearI8(out->data(), xq, xs, wq, ws, bias ? bias->data() : nullptr, t, int(M), int(N), int(Kd), stream());
+}
+
 void rearrange(const tensor_t &out, const tensor_t &in) {
     const char *op = "rearrange";
     LLAISYS_CHECK(out && in, op << ": null tensor");

@@ -130,3 +130,64 @@ class Ops:
         LIB_LLAISYS.llaisysPagedAttentionVarlen(_h(out), _h(q), _h(k_pool), _h(v_pool),
                                                 _h(block_table), _h(cu_q), _h(ctx_len), c_float(scale))
         check_last_error()
+
+    @staticmethod
+    def paged_kv_map(block_table: Tensor, cu_new: Tensor, ctx_after: Tensor, pos_ids: Tensor, slots: Tensor,
+                     ctx_len: Tensor, new_len: Tensor, free_blocks: Tensor = None, free_used: Tensor = None,
+                     free_after: Tensor = None):
+        """A step's block-table entries (from the free list), row offsets, lengths, positions
+        and slots from the sequences' lengths; see llaisysPagedKVMap in include/llaisys/ops.h."""
+        LIB_LLAISYS.llaisysPagedKVMap(_h(block_table), _h(cu_new), _h(ctx_after), _h(pos_ids), _h(slots), _h(ctx_len),
+                                      _h(new_len), _h(free_blocks), _h(free_used), _h(free_after))
+        check_last_error()
+
+    @staticmethod
+    def paged_kv_append_f8(k_pool: Tensor, v_pool: Tensor, k_scale: Tensor, v_scale: Tensor, k_new: Tensor,
+                           v_new: Tensor, slots: Tensor):
+        """Write new K/V rows into the 8-bit pool at their slots (of paged_kv_map); negative slots are skipped."""
+        LIB_LLAISYS.llaisysPagedKVAppendF8(_h(k_pool), _h(v_pool), _h(k_scale), _h(v_scale), _h(k_new), _h(v_new),
+                                           _h(slots))
+        check_last_error()
+
+    @staticmethod
+    def paged_kv_gather_f8(k_out: Tensor, v_out: Tensor, k_pool: Tensor, v_pool: Tensor, k_scale: Tensor,
+                           v_scale: Tensor, block_table: Tensor, cu_seqlens: Tensor):
+        """paged_kv_gather out of the 8-bit pool, as bf16 rows."""
+        LIB_LLAISYS.llaisysPagedKVGatherF8(_h(k_out), _h(v_out), _h(k_pool), _h(v_pool), _h(k_scale), _h(v_scale),
+                                           _h(block_table), _h(cu_seqlens))
+        check_last_error()
+
+    @staticmethod
+    def paged_kv_copy_blocks_f8(k_pool: Tensor, v_pool: Tensor, k_scale: Tensor, v_scale: Tensor, pairs: Tensor):
+        """paged_kv_copy_blocks of the 8-bit pool, scales included."""
+        LIB_LLAISYS.llaisysPagedKVCopyBlocksF8(_h(k_pool), _h(v_pool), _h(k_scale), _h(v_scale), _h(pairs))
+        check_last_error()
+
+    @staticmethod
+    def paged_attention_f8(out: Tensor, q: Tensor, k_pool: Tensor, v_pool: Tensor, k_scale: Tensor, v_scale: Tensor,
+                           block_table: Tensor, ctx_len: Tensor, scale: float):
+        """paged_attention over the 8-bit pool."""
+        LIB_LLAISYS.llaisysPagedAttentionF8(_h(out), _h(q), _h(k_pool), _h(v_pool), _h(k_scale), _h(v_scale),
+                                            _h(block_table), _h(ctx_len), c_float(scale))
+        check_last_error()
+
+    @staticmethod
+    def paged_attention_varlen_f8(out: Tensor, q: Tensor, k_pool: Tensor, v_pool: Tensor, k_scale: Tensor,
+                                  v_scale: Tensor, block_table: Tensor, cu_q: Tensor, ctx_len: Tensor, scale: float):
+        """paged_attention_varlen over the 8-bit pool."""
+        LIB_LLAISYS.llaisysPagedAttentionVarlenF8(_h(out), _h(q), _h(k_pool), _h(v_pool), _h(k_scale), _h(v_scale),
+                                                  _h(block_table), _h(cu_q), _h(ctx_len), c_float(scale))
+        check_last_error()
+
+    @staticmethod
+    def quantize_rows(q: Tensor, scale: Tensor, x: Tensor):
+        """Rows of x as 8-bit integers q with a scale each (the largest magnitude is 127)."""
+        LIB_LLAISYS.llaisysQuantizeRows(_h(q), _h(scale), _h(x))
+        check_last_error()
+
+    @staticmethod
+    def linear_i8(out: Tensor, inp: Tensor, inp_scale: Tensor, weight: Tensor, weight_scale: Tensor,
+                  bias: Tensor = None):
+        """out = (inp . weight^T) * (inp_scale[:, None] * weight_scale) + bias over 8-bit integers."""
+        LIB_LLAISYS.llaisysLinearI8(_h(out), _h(inp), _h(inp_scale), _h(weight), _h(weight_scale), _h(bias))
+        check_last_error()
