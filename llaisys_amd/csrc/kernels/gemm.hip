@@ -46,6 +46,7 @@
 #include <algorithm>
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 namespace llaisys::kernels {
@@ -55,6 +56,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kXcds = 8;
@@ -68,11 +70,19 @@ template <ElemType T> struct Elem;
 template <> struct Elem<ElemType::BF16> { using type = __bf16; static constexpr int size = 2; };
 template <> struct Elem<ElemType::F16> { using type = _Float16; static constexpr int size = 2; };
 template <> struct Elem<ElemType::F32> { using type = float; static constexpr int size = 4; };
+// Operands of 8-bit integers (linearI8), inside this file only; their sums are
+// 32-bit integers and their results, of type O, floats.
+constexpr ElemType kI8 = ElemType(3);
+template <> struct Elem<kI8> { using type = int8_t; static constexpr int size = 1; };
+template <ElemType T> using AccOf = std::conditional_t<T == kI8, i32x4, f32x4>;
 
-// acc += A . B for one 16 B piece per lane (one 32-k step for 16-bit types,
-// one 16-k step for f32).
-template <ElemType T> __device__ __forceinline__ f32x4 mfmaPiece(u32x4 a, u32x4 b, f32x4 acc) {
-    if constexpr (T == ElemType::BF16) {
+// acc += A . B for one 16 B piece per lane (one 64-k step for 8-bit integers,
+// 32-k for 16-bit types, 16-k for f32).
+template <ElemType T> __device__ __forceinline__ AccOf<T> mfmaPiece(u32x4 a, u32x4 b, AccOf<T> acc) {
+    if constexpr (T == kI8) {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), acc, 0,
+                                                     0, 0);
+    } else if constexpr (T == ElemType::BF16) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
                                                        acc, 0, 0, 0);
     } else if constexpr (T == ElemType::F16) {
@@ -118,9 +128,15 @@ template <ElemType T> __device__ __forceinline__ void store4(void *p, size_t i, 
     }
 }
 
+// Sums as floats (integers rounded to 24 bits: 2^-24 of the result at most).
+template <ElemType T> __device__ __forceinline__ f32x4 floats(AccOf<T> v) {
+    return f32x4{float(v[0]), float(v[1]), float(v[2]), float(v[3])};
+}
+
 struct GemmParams {
     void *y;
     const void *x, *w, *bias;
+    const float *xs, *ws; // 8-bit integers: scales of the rows of x and of w
     int M, N, K;
     int accumulate;
     int mtiles, ntiles;
@@ -208,7 +224,8 @@ template <int BM, int BN, int NW> constexpr int wideStages() {
 // before it to land; the second step's fragments are read under the first
 // step's MFMAs.
 // WGM x WGN waves, wave (wm, wn) owning the (BM / WGM) x (BN / WGN) sub-tile.
-template <ElemType T, int BM, int BN, int WGM = 2, int WGN = 2, bool PIPE = false, int RB = 64, int WS = 2>
+template <ElemType T, int BM, int BN, int WGM = 2, int WGN = 2, bool PIPE = false, int RB = 64, int WS = 2,
+          ElemType O = T>
 __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
     static_assert(RB == 64 || RB == 128, "k tiles of 64 or 128 B per row");
     constexpr bool WIDE = RB == 128;
@@ -272,11 +289,11 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
         for (int l = 0; l < kLoadsPerStage; ++l) issueOne(kt, l);
     };
 
-    f32x4 acc[TN][TM];
+    AccOf<T> acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TM; ++j) acc[i][j] = AccOf<T>{0, 0, 0, 0};
 
 #pragma unroll
     for (int s = 0; s < (WIDE ? NS : NS - 1); ++s) issue(s);
@@ -464,10 +481,12 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
     // Epilogue: lane holds Y[m][n .. n + 3], m = row l % 16 of X fragment j,
     // n = 4 (l / 16) of W fragment i; (old Y +) sum (+ bias), rounded once;
     // or, split, the fp32 partial for the reduce.
+    // (8-bit integers: the sum times the scales of its row and column.)
     const int fg = lane >> 4;
     const bool vec = (p.N & 3) == 0;
     if (p.splits > 1) {
-        float *part = p.part + size_t(split) * p.M * p.N;
+        typename std::conditional<T == kI8, int, float>::type *part = nullptr;
+        part = reinterpret_cast<decltype(part)>(p.part) + size_t(split) * p.M * p.N;
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
             const int m = m0 + wm * (BM / WGM) + 16 * j + fr;
@@ -478,7 +497,7 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
                 if (n >= p.N) continue;
                 const size_t base = size_t(m) * p.N + n;
                 if (vec) {
-                    *reinterpret_cast<f32x4 *>(part + base) = acc[i][j];
+                    *reinterpret_cast<AccOf<T> *>(part + base) = acc[i][j];
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -488,14 +507,14 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
         }
         return;
     }
-    if constexpr (ES == 2) {
+    if constexpr (Elem<O>::size == 2) {
         if (p.staged) {
             // The tile leaves through LDS (the ring is idle now): every lane
             // writes its 8 B pieces to a row-major copy, then each lane stores
             // 16 B of a row, so one store instruction writes whole 128 B lines
             // (the fragment layout writes 32 B of 16 rows each, and the stores
             // then took a fifth of a 256 x 256 x 1536 tile's time).
-            using E = typename Elem<T>::type;
+            using E = typename Elem<O>::type;
             typedef E e4 __attribute__((ext_vector_type(4)));
             constexpr int PITCH = stagePitch<BN>();
             char *stage = reinterpret_cast<char *>(lds);
@@ -530,13 +549,15 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
 #pragma unroll
                 for (int j = 0; j < TM; ++j) {
                     const int ml = wm * (BM / WGM) + 16 * j + fr, m = m0 + ml;
+                    const float xs = T == kI8 && m < p.M ? p.xs[m] : 0.f;
 #pragma unroll
                     for (int i = 0; i < TN; ++i) {
                         const int nl = wn * (BN / WGN) + 16 * i + 4 * fg, n = n0 + nl;
-                        f32x4 v = acc[i][j];
+                        f32x4 v = floats<T>(acc[i][j]);
                         if (m < p.M && n < p.N) {
-                            if (p.accumulate) v = load4<T>(p.y, size_t(m) * p.ldy + n) + v;
-                            if (p.bias) v += load4<T>(p.bias, n);
+                            if constexpr (T == kI8) v *= xs * load4<ElemType::F32>(p.ws, n);
+                            if (p.accumulate) v = load4<O>(p.y, size_t(m) * p.ldy + n) + v;
+                            if (p.bias) v += load4<O>(p.bias, n);
                         }
                         *reinterpret_cast<e4 *>(stage + ml * PITCH + nl * 2) = e4{E(v[0]), E(v[1]), E(v[2]), E(v[3])};
                     }
@@ -607,19 +628,21 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemmKernel(GemmParams p) {
             const int n = n0 + wn * (BN / WGN) + 16 * i + 4 * fg;
             if (n >= p.N) continue;
             const size_t base = size_t(m) * p.ldy + n;
-            f32x4 v = acc[i][j];
+            f32x4 v = floats<T>(acc[i][j]);
             if (vec) {
-                if (p.accumulate) v = load4<T>(p.y, base) + v;
-                if (p.bias) v += load4<T>(p.bias, n);
-                store4<T>(p.y, base, v);
+                if constexpr (T == kI8) v *= p.xs[m] * load4<ElemType::F32>(p.ws, n);
+                if (p.accumulate) v = load4<O>(p.y, base) + v;
+                if (p.bias) v += load4<O>(p.bias, n);
+                store4<O>(p.y, base, v);
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     if (n + r >= p.N) break;
                     float e = v[r];
-                    if (p.accumulate) e = loadElem<T>(p.y, base + r) + e;
-                    if (p.bias) e += loadElem<T>(p.bias, n + r);
-                    storeElem<T>(p.y, base + r, e);
+                    if constexpr (T == kI8) e *= p.xs[m] * p.ws[n + r];
+                    if (p.accumulate) e = loadElem<O>(p.y, base + r) + e;
+                    if (p.bias) e += loadElem<O>(p.bias, n + r);
+                    storeElem<O>(p.y, base + r, e);
                 }
             }
         }
@@ -667,6 +690,33 @@ __global__ void __launch_bounds__(256) gemmReduceKernel(void *y, const float *pa
     }
 }
 
+// The same of 8-bit integers' partial sums: exact, then the scales.
+template <ElemType O>
+__global__ void __launch_bounds__(256)
+    gemmReduceI8Kernel(void *y, const int *part, const float *xs, const float *ws, const void *bias, int M, int N,
+                       int S) {
+    const size_t idx = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    const size_t stride = size_t(M) * N;
+    if ((N & 3) == 0) {
+        if (idx >= stride / 4) return;
+        const size_t base = 4 * idx;
+        const int m = int(base / N), n = int(base - size_t(m) * N);
+        i32x4 sum = *reinterpret_cast<const i32x4 *>(part + base);
+        for (int s = 1; s < S; ++s) sum += *reinterpret_cast<const i32x4 *>(part + s * stride + base);
+        f32x4 v = floats<kI8>(sum) * (xs[m] * load4<ElemType::F32>(ws, n));
+        if (bias) v += load4<O>(bias, n);
+        store4<O>(y, base, v);
+    } else {
+        if (idx >= stride) return;
+        const int m = int(idx / N), n = int(idx - size_t(m) * N);
+        int sum = part[idx];
+        for (int s = 1; s < S; ++s) sum += part[s * stride + idx];
+        float v = float(sum) * (xs[m] * ws[n]);
+        if (bias) v += loadElem<O>(bias, n);
+        storeElem<O>(y, idx, v);
+    }
+}
+
 // Few rows of X (M <= 16 MT): W is streamed once by many small workgroups and
 // nothing is staged. A workgroup of NW waves owns R rows of W; its waves take
 // the rows' 128 B segments in turn, straight from memory into MFMA operands.
@@ -675,11 +725,12 @@ __global__ void __launch_bounds__(256) gemmReduceKernel(void *y, const float *pa
 // and column group a meet in the quadrants (a, a), the others are unused, and
 // a workgroup owns fewer rows, so that more of them share a narrow W. The
 // NW KR partial sums of an output meet in LDS in a fixed order.
-template <ElemType T, int R, int NW, int MT>
+template <ElemType T, int R, int NW, int MT, ElemType O = T>
 __global__ void __launch_bounds__(64 * NW) gemmFewRowsKernel(GemmParams p) {
     static_assert(MT == 1 || R == 16, "column groups are of one tile");
     constexpr int KR = 16 / R, U = MT == 1 ? 4 : 2; // segments in flight per set
-    __shared__ float part[NW * KR][MT * R][R];
+    using Sum = std::conditional_t<T == kI8, int, float>;
+    __shared__ Sum part[NW * KR][MT * R][R];
     const int lane = threadIdx.x & 63, n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = int(blockIdx.x) * R;
@@ -713,11 +764,11 @@ __global__ void __launch_bounds__(64 * NW) gemmFewRowsKernel(GemmParams p) {
     // f32: a sum per segment of a set, so that the chains of additions stay
     // short (16 x 2048 x 1536: error 3.6e-7 -> 1.9e-7 of the result's 2-norm).
     constexpr int SUMS = T == ElemType::F32 ? U : 1;
-    f32x4 acc[SUMS][MT];
+    AccOf<T> acc[SUMS][MT];
 #pragma unroll
     for (int u = 0; u < SUMS; ++u)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < MT; ++t) acc[u][t] = AccOf<T>{0, 0, 0, 0};
     auto use = [&](const Set &f) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -744,19 +795,21 @@ __global__ void __launch_bounds__(64 * NW) gemmFewRowsKernel(GemmParams p) {
     if ((4 * grp) / R == n / R) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
-            *reinterpret_cast<f32x4 *>(&part[wave * KR + n / R][t * R + n % R][(4 * grp) % R]) = acc[0][t];
+            *reinterpret_cast<AccOf<T> *>(&part[wave * KR + n / R][t * R + n % R][(4 * grp) % R]) = acc[0][t];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < MT * R * R; i += 64 * NW) {
         const int m = i / R, r = i % R;
         if (m >= p.M || n0 + r >= p.N) continue;
-        float v = part[0][m][r];
+        Sum sum = part[0][m][r];
 #pragma unroll
-        for (int s = 1; s < NW * KR; ++s) v += part[s][m][r];
+        for (int s = 1; s < NW * KR; ++s) sum += part[s][m][r];
+        float v = float(sum);
+        if constexpr (T == kI8) v *= p.xs[m] * p.ws[n0 + r];
         const size_t at = size_t(m) * p.ldy + n0 + r;
-        if (p.accumulate) v = loadElem<T>(p.y, at) + v;
-        if (p.bias) v += loadElem<T>(p.bias, n0 + r);
-        storeElem<T>(p.y, at, v);
+        if (p.accumulate) v = loadElem<O>(p.y, at) + v;
+        if (p.bias) v += loadElem<O>(p.bias, n0 + r);
+        storeElem<O>(p.y, at, v);
     }
 }
 
@@ -771,10 +824,10 @@ int cusOf() {
     return cache[dev];
 }
 
-template <ElemType T, int BM, int BN, int WGM, int WGN, bool PIPE, int RB = 64, int WS = 2>
+template <ElemType T, int BM, int BN, int WGM, int WGN, bool PIPE, int RB = 64, int WS = 2, ElemType O = T>
 void launchTileAs(GemmParams p, hipStream_t s) {
     const size_t lds = std::max(size_t(ringStages<PIPE, RB, WS>()) * stageBlocks<BM, BN, WGM * WGN, RB>() * 1024,
-                                Elem<T>::size == 2 ? stageBytes<BM, BN>() : size_t(0));
+                                Elem<O>::size == 2 ? stageBytes<BM, BN>() : size_t(0));
     // The LDS limit is raised once per device the kernel runs on.
     static std::mutex mu;
     static std::vector<bool> raised;
@@ -784,12 +837,12 @@ void launchTileAs(GemmParams p, hipStream_t s) {
         std::lock_guard<std::mutex> lock(mu);
         if (size_t(dev) >= raised.size()) raised.resize(dev + 1, false);
         if (!raised[dev]) {
-            HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemmKernel<T, BM, BN, WGM, WGN, PIPE, RB, WS>),
+            HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemmKernel<T, BM, BN, WGM, WGN, PIPE, RB, WS, O>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
             raised[dev] = true;
         }
     }
-    hipLaunchKernelGGL((gemmKernel<T, BM, BN, WGM, WGN, PIPE, RB, WS>), dim3(unsigned(p.mtiles * p.ntiles * p.splits)),
+    hipLaunchKernelGGL((gemmKernel<T, BM, BN, WGM, WGN, PIPE, RB, WS, O>), dim3(unsigned(p.mtiles * p.ntiles * p.splits)),
                        dim3(64 * WGM * WGN), lds, s, p);
 }
 
@@ -807,7 +860,12 @@ bool wideK() {
     return v;
 }
 
-template <ElemType T, int BM, int BN, int WGM = 2, int WGN = 2> void launchTile(GemmParams p, hipStream_t s) {
+template <ElemType T, int BM, int BN, int WGM = 2, int WGN = 2, ElemType O = T>
+void launchTile(GemmParams p, hipStream_t s) {
+    if constexpr (T == kI8) {
+        launchTileAs<T, BM, BN, WGM, WGN, true, 128, wideStages<BM, BN, WGM * WGN>(), O>(p, s);
+        return;
+    }
     if constexpr (Elem<T>::size == 2) {
         if (wideK()) {
             static const bool deep = [] { const char *e = std::getenv("LLAISYS_GEMM_WIDE_DEEP"); return !(e && e[0] == '0'); }();
@@ -818,10 +876,12 @@ template <ElemType T, int BM, int BN, int WGM = 2, int WGN = 2> void launchTile(
             return;
         }
     }
-    if (pipelined())
-        launchTileAs<T, BM, BN, WGM, WGN, true>(p, s);
-    else
-        launchTileAs<T, BM, BN, WGM, WGN, false>(p, s);
+    if constexpr (T != kI8) {
+        if (pipelined())
+            launchTileAs<T, BM, BN, WGM, WGN, true>(p, s);
+        else
+            launchTileAs<T, BM, BN, WGM, WGN, false>(p, s);
+    }
 }
 
 // The (tile, K split) with the least estimated time. A launch runs
@@ -989,59 +1049,64 @@ bool takesFewRows(ElemType t, const GemmParams &p) {
     return p.M <= 32 && p.K <= 2048 && nk <= (1L << 22);
 }
 
-template <ElemType T, int R, int NW, int MT> void launchFewRowsAs(const GemmParams &p, hipStream_t s) {
-    hipLaunchKernelGGL((gemmFewRowsKernel<T, R, NW, MT>), dim3(unsigned((p.N + R - 1) / R)), dim3(64 * NW), 0, s, p);
+template <ElemType T, int R, int NW, int MT, ElemType O = T>
+void launchFewRowsAs(const GemmParams &p, hipStream_t s) {
+    hipLaunchKernelGGL((gemmFewRowsKernel<T, R, NW, MT, O>), dim3(unsigned((p.N + R - 1) / R)), dim3(64 * NW), 0, s, p);
     HIP_CHECK(hipGetLastError());
 }
 
 // 2 waves a workgroup for the 16-bit rows of M <= 4, else 4 (8 were slower on
 // wide W: half of them had no segment at K = 1536).
-template <ElemType T> void launchFewRows(const GemmParams &p, hipStream_t s) {
-    if (p.M <= 4) launchFewRowsAs<T, 4, Elem<T>::size == 4 ? 4 : 2, 1>(p, s);
-    else if (p.M <= 8) launchFewRowsAs<T, 8, 4, 1>(p, s);
-    else if (p.M <= 16) launchFewRowsAs<T, 16, 4, 1>(p, s);
-    else launchFewRowsAs<T, 16, 4, 2>(p, s);
+template <ElemType T, ElemType O = T> void launchFewRows(const GemmParams &p, hipStream_t s) {
+    if (p.M <= 4) launchFewRowsAs<T, 4, Elem<T>::size == 4 ? 4 : 2, 1, O>(p, s);
+    else if (p.M <= 8) launchFewRowsAs<T, 8, 4, 1, O>(p, s);
+    else if (p.M <= 16) launchFewRowsAs<T, 16, 4, 1, O>(p, s);
+    else launchFewRowsAs<T, 16, 4, 2, O>(p, s);
 }
 
-template <ElemType T> void launchGemm(GemmParams p, const Plan &plan, hipStream_t s) {
+template <ElemType T, ElemType O = T> void launchGemm(GemmParams p, const Plan &plan, hipStream_t s) {
     p.mtiles = plan.mtiles;
     p.ntiles = plan.ntiles;
     p.splits = plan.splits;
     switch (plan.tile) {
     case 0:
-        if (w8()) launchTile<T, 128, 256, 2, 4>(p, s);
-        else launchTile<T, 128, 256>(p, s);
+        if (T == kI8 || w8()) launchTile<T, 128, 256, 2, 4, O>(p, s);
+        else if constexpr (T != kI8) launchTile<T, 128, 256>(p, s);
         break;
     case 1:
-        if (w8()) launchTile<T, 256, 128, 4, 2>(p, s);
-        else launchTile<T, 256, 128>(p, s);
+        if (T == kI8 || w8()) launchTile<T, 256, 128, 4, 2, O>(p, s);
+        else if constexpr (T != kI8) launchTile<T, 256, 128>(p, s);
         break;
-    case 2: launchTile<T, 128, 128>(p, s); break;
+    case 2: launchTile<T, 128, 128, 2, 2, O>(p, s); break;
     case 4:
         if constexpr (T != ElemType::F32) {
-            launchTile<T, 256, 256, 2, 4>(p, s);
+            launchTile<T, 256, 256, 2, 4, O>(p, s);
             break;
         }
         [[fallthrough]];
     case kTile192:
         if constexpr (T != ElemType::F32) {
-            launchTile<T, 256, 192, 2, 4>(p, s);
+            launchTile<T, 256, 192, 2, 4, O>(p, s);
             break;
         }
         [[fallthrough]];
     case kTile96:
         if constexpr (T != ElemType::F32) {
-            launchTile<T, 128, 96>(p, s);
+            launchTile<T, 128, 96, 2, 2, O>(p, s);
             break;
         }
         [[fallthrough]];
-    default: launchTile<T, 64, 64>(p, s); break;
+    default: launchTile<T, 64, 64, 2, 2, O>(p, s); break;
     }
     HIP_CHECK(hipGetLastError());
     if (plan.splits > 1) {
         const size_t n = (p.N & 3) == 0 ? size_t(p.M) * p.N / 4 : size_t(p.M) * p.N;
-        hipLaunchKernelGGL(gemmReduceKernel<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, p.y, p.part, p.bias,
-                           p.M, p.N, plan.splits, p.accumulate);
+        if constexpr (T == kI8)
+            hipLaunchKernelGGL(gemmReduceI8Kernel<O>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, p.y,
+                               reinterpret_cast<const int *>(p.part), p.xs, p.ws, p.bias, p.M, p.N, plan.splits);
+        else
+            hipLaunchKernelGGL(gemmReduceKernel<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, p.y, p.part,
+                               p.bias, p.M, p.N, plan.splits, p.accumulate);
         HIP_CHECK(hipGetLastError());
     }
 }
@@ -1159,6 +1224,113 @@ void linear(void *y, const void *x, const void *w, const void *bias, ElemType t,
         } else {
             run(0, N, plan);
         }
+    }
+}
+
+namespace {
+
+// Rows that are not whole 16 B pieces: one thread per output.
+template <ElemType O>
+__global__ void __launch_bounds__(256) gemmRowsI8Kernel(GemmParams p) {
+    const size_t idx = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (idx >= size_t(p.M) * p.N) return;
+    const int m = int(idx / p.N), n = int(idx % p.N);
+    const int8_t *x = static_cast<const int8_t *>(p.x) + size_t(m) * p.K;
+    const int8_t *w = static_cast<const int8_t *>(p.w) + size_t(n) * p.K;
+    int sum = 0;
+    for (int k = 0; k < p.K; ++k) sum += int(x[k]) * int(w[k]);
+    float v = float(sum) * (p.xs[m] * p.ws[n]);
+    if (p.bias) v += loadElem<O>(p.bias, n);
+    storeElem<O>(p.y, idx, v);
+}
+
+// 8-bit operands move and multiply as 16-bit ones of half the K do (the same
+// bytes, and a 64-k step of them takes an MFMA the time of a 32-k one), so the
+// 16-bit plans and lines are theirs at K / 2.
+bool tiledI8(const void *x, const void *w, int K) {
+    return K > 0 && K % 16 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) % 16 == 0;
+}
+
+template <ElemType O>
+void linearI8As(void *y, const int8_t *x, const float *xs, const int8_t *w, const float *ws, const void *bias, int M,
+                int N, int K, void *workspace, hipStream_t s) {
+    constexpr int es = Elem<O>::size;
+    GemmParams p{};
+    p.w = w;
+    p.ws = ws;
+    p.bias = bias;
+    p.N = N;
+    p.K = K;
+    p.ldy = N;
+    if (!tiledI8(x, w, K)) {
+        p.y = y;
+        p.x = x;
+        p.xs = xs;
+        p.M = M;
+        hipLaunchKernelGGL(gemmRowsI8Kernel<O>, dim3(unsigned((size_t(M) * N + 255) / 256)), dim3(256), 0, s, p);
+        HIP_CHECK(hipGetLastError());
+        return;
+    }
+    const int rows_per_launch = rowsPerLaunch(ElemType::BF16, M, K / 2);
+    for (int r0 = 0; r0 < M; r0 += rows_per_launch) {
+        const int m = std::min(rows_per_launch, M - r0);
+        p.M = m;
+        p.xs = xs + r0;
+        p.x = x + size_t(r0) * K;
+        p.x_bytes = uint32_t(size_t(m) * K);
+        auto columns = [&](int c0, int c1) {
+            GemmParams q = p;
+            q.y = static_cast<char *>(y) + (size_t(r0) * N + c0) * es;
+            q.w = w + size_t(c0) * K;
+            q.ws = ws + c0;
+            q.bias = bias ? static_cast<const char *>(bias) + size_t(c0) * es : nullptr;
+            q.N = c1 - c0;
+            q.w_bytes = uint32_t(size_t(c1 - c0) * K);
+            q.part = static_cast<float *>(workspace);
+            return q;
+        };
+        if (m <= 32) {
+            GemmParams lines = columns(0, N);
+            lines.K = K / 2;
+            if (takesFewRows(ElemType::BF16, lines)) {
+                launchFewRows<kI8, O>(columns(0, N), s);
+                continue;
+            }
+        }
+        const Plan plan = planGemm(ElemType::BF16, m, N, K / 2);
+        LLAISYS_CHECK(plan.splits == 1 || workspace, "linearI8: this shape needs linearI8WorkspaceBytes() of workspace");
+        auto run = [&](int c0, int c1, const Plan &pl) {
+            GemmParams q = columns(c0, c1);
+            q.staged = es == 2 && pl.splits == 1 && N % 8 == 0 && (c1 - c0) % 8 == 0 &&
+                       reinterpret_cast<uintptr_t>(q.y) % 16 == 0 && stagedStores();
+            launchGemm<kI8, O>(q, pl, s);
+        };
+        const ColumnSplit cs = splitColumns(ElemType::BF16, m, N, K / 2, plan);
+        if (cs.na) {
+            run(0, cs.na, cs.a);
+            run(cs.na, N, cs.b);
+        } else {
+            run(0, N, plan);
+        }
+    }
+}
+
+} // namespace
+
+size_t linearI8WorkspaceBytes(const int8_t *x, const int8_t *w, int M, int N, int K) {
+    return tiledI8(x, w, K) ? linearWorkspaceBytes(ElemType::BF16, M, N, K / 2) : 0;
+}
+
+void linearI8(void *y, const int8_t *x, const float *xs, const int8_t *w, const float *ws, const void *bias, ElemType t,
+              int M, int N, int K, void *stream, void *workspace) {
+    if (M <= 0 || N <= 0) return;
+    LLAISYS_CHECK(size_t(N) * K < kMaxBufferBytes || !tiledI8(x, w, K),
+                  "linear_i8: the weight (" << N << " x " << K << ") must be under 2 GiB");
+    auto s = static_cast<hipStream_t>(stream);
+    switch (t) {
+    case ElemType::BF16: linearI8As<ElemType::BF16>(y, x, xs, w, ws, bias, M, N, K, workspace, s); break;
+    case ElemType::F16: linearI8As<ElemType::F16>(y, x, xs, w, ws, bias, M, N, K, workspace, s); break;
+    case ElemType::F32: linearI8As<ElemType::F32>(y, x, xs, w, ws, bias, M, N, K, workspace, s); break;
     }
 }
 

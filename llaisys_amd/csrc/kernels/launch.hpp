@@ -172,16 +172,18 @@ void pagedAttentionF8(void *out, bool out_f32, const uint16_t *q, const uint8_t 
                       const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
                       int *err, void *stream);
 
-// ---- 8-bit integers (quant.hip)
+// ---- 8-bit integers (quant.hip, gemm.hip)
 // scale[m] = max |x[m, :]| / 127 and q[m, k] = x[m, k] / scale[m] to the
 // nearest whole number (ties to even); a row with a value that is not finite
 // gets the scale NaN and zeros.
 void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K, void *stream);
-// y[M, N] = (xq . wq^T) * (xs[m] * ws[n]) (+ bias[n]), the products summed in
-// 32-bit integers (K <= kLinearI8MaxK), one rounding to t.
+// y[M, N] = (x . w^T) * (xs[m] * ws[n]) (+ bias[n]) for x [M, K], w [N, K]
+// (gemm.hip), the products summed in 32-bit integers (K <= kLinearI8MaxK), one
+// rounding to t. Split K leaves integer partials in `workspace`.
 constexpr int kLinearI8MaxK = 131071; // 128 * 128 * K < 2^31
-void linearI8(void *y, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const void *bias,
-              ElemType t, int M, int N, int K, void *stream);
+size_t linearI8WorkspaceBytes(const int8_t *x, const int8_t *w, int M, int N, int K);
+void linearI8(void *y, const int8_t *x, const float *xs, const int8_t *w, const float *ws, const void *bias, ElemType t,
+              int M, int N, int K, void *stream, void *workspace);
 
 // ---- model ops (model_ops.hip, linear.cpp)
 constexpr int kMaxDims = 8;

@@ -62,22 +62,6 @@ __global__ void __launch_bounds__(256) quantizeRowsKernel(int8_t *__restrict__ q
     for (int k = lane; k < K; k += 64) to[k] = some ? int8_t(quantized(float(row[k]) * grow, sg, inv)) : int8_t(0);
 }
 
-template <ElemType T>
-__global__ void __launch_bounds__(256)
-    linearI8RowsKernel(void *y, const int8_t *__restrict__ xq, const float *__restrict__ xs,
-                       const int8_t *__restrict__ wq, const float *__restrict__ ws, const void *bias, int M, int N,
-                       int K) {
-    using E = typename Elem<T>::type;
-    const size_t idx = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (idx >= size_t(M) * N) return;
-    const int m = int(idx / N), n = int(idx % N);
-    int sum = 0;
-    for (int k = 0; k < K; ++k) sum += int(xq[size_t(m) * K + k]) * int(wq[size_t(n) * K + k]);
-    float v = float(sum) * (xs[m] * ws[n]);
-    if (bias) v += float(static_cast<const E *>(bias)[n]);
-    static_cast<E *>(y)[idx] = E(v);
-}
-
 } // namespace
 
 void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K, void *stream) {
@@ -88,19 +72,6 @@ void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int
     case ElemType::F32: hipLaunchKernelGGL(quantizeRowsKernel<ElemType::F32>, grid, block, 0, s, q, scale, x, M, K); break;
     case ElemType::F16: hipLaunchKernelGGL(quantizeRowsKernel<ElemType::F16>, grid, block, 0, s, q, scale, x, M, K); break;
     case ElemType::BF16: hipLaunchKernelGGL(quantizeRowsKernel<ElemType::BF16>, grid, block, 0, s, q, scale, x, M, K); break;
-    }
-    HIP_CHECK(hipGetLastError());
-}
-
-void linearI8(void *y, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const void *bias,
-              ElemType t, int M, int N, int K, void *stream) {
-    if (M == 0 || N == 0) return;
-    const dim3 grid(unsigned((size_t(M) * N + 255) / 256)), block(256);
-    auto s = static_cast<hipStream_t>(stream);
-    switch (t) {
-    case ElemType::F32: hipLaunchKernelGGL(linearI8RowsKernel<ElemType::F32>, grid, block, 0, s, y, xq, xs, wq, ws, bias, M, N, K); break;
-    case ElemType::F16: hipLaunchKernelGGL(linearI8RowsKernel<ElemType::F16>, grid, block, 0, s, y, xq, xs, wq, ws, bias, M, N, K); break;
-    case ElemType::BF16: hipLaunchKernelGGL(linearI8RowsKernel<ElemType::BF16>, grid, block, 0, s, y, xq, xs, wq, ws, bias, M, N, K); break;
     }
     HIP_CHECK(hipGetLastError());
 }

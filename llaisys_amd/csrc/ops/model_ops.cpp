@@ -224,7 +224,9 @@ void linearI8(const tensor_t &out, const tensor_t &in, const tensor_t &in_scale,
     const auto *ws = reinterpret_cast<const float *>(weight_scale->data());
     if (host)
         return C::linearI8(out->data(), xq, xs, wq, ws, bias ? bias->data() : nullptr, t, int(M), int(N), int(Kd));
-    K::linearI8(out->data(), xq, xs, wq, ws, bias ? bias->data() : nullptr, t, int(M), int(N), int(Kd), stream());
+    void *space = core::context().runtime().scratch(K::linearI8WorkspaceBytes(xq, wq, int(M), int(N), int(Kd)));
+    K::linearI8(out->data(), xq, xs, wq, ws, bias ? bias->data() : nullptr, t, int(M), int(N), int(Kd), stream(),
+                space);
 }
 
 void rearrange(const tensor_t &out, const tensor_t &in) {
