@@ -55,11 +55,14 @@ struct DecodePlan {
     size_t slot_record_bytes; // per-unit record slots
 };
 constexpr int kDecodeMaxBatch = 4096; // sequences per launch (LDS-resident prefix)
-DecodePlan planDecode(int B, int nkvh, int group, int max_pages);
+// 8-bit pages (here and in pagedDecodeUnits and pagedPrefill): the pools are
+// bytes, with k_scale and v_scale; bf16 outputs are not packed then.
+DecodePlan planDecode(int B, int nkvh, int group, int max_pages, bool f8 = false);
 void pagedDecode(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
                  const int32_t *block_table, const int32_t *ctx_len, const int32_t *cu_q, int B, int T, int nh,
                  int nkvh, int max_pages, int num_blocks, float scale, const DecodePlan &plan, float *records,
-                 int *err, int *slot_headers, void *slot_records, void *stream, uint16_t *out_packed = nullptr);
+                 int *err, int *slot_headers, void *slot_records, void *stream, uint16_t *out_packed = nullptr,
+                 const float *k_scale = nullptr, const float *v_scale = nullptr);
 
 // The same attention (cu_q null: query row b is sequence b) with one
 // workgroup of 4 waves per (sequence, kv head), merging in LDS: no records,
@@ -71,7 +74,7 @@ void pagedDecode(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_p
 void pagedDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
                       const int32_t *block_table, const int32_t *ctx_len, int B, int nh, int nkvh, int max_pages,
                       int num_blocks, float scale, int *err, void *stream, uint16_t *out_packed = nullptr,
-                      bool keep_invalid = false);
+                      bool keep_invalid = false, const float *k_scale = nullptr, const float *v_scale = nullptr);
 // Whether a batch of contexts of up to max_pages pages takes it whatever their
 // spread (the host knows the table's width, not the lengths): one launch
 // instead of two while a unit is short (us, this / stream-K in a wider table,
@@ -140,7 +143,8 @@ constexpr int kPrefillQueueWords = 33;
 void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
                   const int32_t *block_table, const int32_t *ctx_len, const int32_t *cu_q, int B, int T, int nh,
                   int nkvh, int max_pages, int num_blocks, float scale, const PagedAttentionPlan &plan,
-                  float *records, int *err, int *queue, void *stream);
+                  float *records, int *err, int *queue, void *stream, const float *k_scale = nullptr,
+                  const float *v_scale = nullptr);
 
 // ---- a step's tables (paged_map.hip)
 // Per sequence its c = ctx_len and n = new_len: cu_new the prefix sums of n (at
@@ -165,12 +169,6 @@ void pagedGatherF8(uint16_t *k_out, uint16_t *v_out, const uint8_t *k_pool, cons
                    int T, int B, int nkvh, int max_pages, int num_blocks, int *err, void *stream);
 void pagedCopyBlocksF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const int32_t *pairs, int P,
                        int nkvh, int num_blocks, int *err, void *stream);
-// Attention over it, one query per sequence (cu_q null, T == B) or sequence b's
-// rows [cu_q[b], cu_q[b + 1]), causal.
-void pagedAttentionF8(void *out, bool out_f32, const uint16_t *q, const uint8_t *k_pool, const uint8_t *v_pool,
-                      const float *k_scale, const float *v_scale, const int32_t *block_table, const int32_t *ctx_len,
-                      const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
-                      int *err, void *stream);
 
 // ---- 8-bit integers (quant.hip, gemm.hip)
 // scale[m] = max |x[m, :]| / 127 and q[m, k] = x[m, k] / scale[m] to the

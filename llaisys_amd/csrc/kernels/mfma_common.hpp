@@ -17,6 +17,7 @@
 // Nothing crosses lanes except the running max (2 shuffles).
 #pragma once
 
+#include "f8_page.hpp"
 #include "lanes.hpp"
 #include "launch.hpp"
 
@@ -295,6 +296,93 @@ __device__ __forceinline__ void consumePair(Acc &acc, PagePair &r, const u32x4 (
     maskStaleV(r.va, r.vb, first_key, ctx, hasB, grp);
     accumulatePV<PARTS>(acc, r.va, r.vb, P);
 }
+
+// Two of a word's four e4m3 codes (the high two: HI) times a power of two, as
+// bf16: exact, one instruction.
+template <bool HI> __device__ __forceinline__ uint32_t widen2(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+// Half h of an 8-bit page (one load) as quarters 2h and 2h + 1 of the bf16 page.
+__device__ __forceinline__ void widenHalf(u32x4 &q0, u32x4 &q1, u32x4 c, float scale) {
+    q0 = u32x4{widen2<false>(c[0], scale), widen2<true>(c[0], scale), widen2<false>(c[1], scale),
+               widen2<true>(c[1], scale)};
+    q1 = u32x4{widen2<false>(c[2], scale), widen2<true>(c[2], scale), widen2<false>(c[3], scale),
+               widen2<true>(c[3], scale)};
+}
+
+// The two kinds of page that the attention kernels read: a page pair's
+// registers, its loads (page bases in u32x4 units, lane offset applied) and the
+// step that consumes it. The 8-bit one is widened to the bf16 one's operands,
+// so the rest is the same.
+struct PairScales {
+    float ka, kb, va, vb;
+};
+struct KvBf16 {
+    static constexpr bool kScaled = false;
+    static constexpr int kPageVecs = kPageElems * 2 / 16;
+    using Pair = PagePair;
+    static __device__ __forceinline__ void load(Pair &r, const u32x4 *kp, const u32x4 *vp, size_t oa, size_t ob) {
+        loadPair(r, kp, vp, oa, ob);
+    }
+    template <int PARTS>
+    static __device__ __forceinline__ void consume(Acc &acc, Pair &r, const PairScales &, const u32x4 (&qop)[4],
+                                                   int first_key, int pos, int ctx, bool hasB, int grp,
+                                                   float scale_log2) {
+        consumePair<PARTS>(acc, r, qop, first_key, pos, ctx, hasB, grp, scale_log2);
+    }
+};
+struct KvF8 {
+    static constexpr bool kScaled = true;
+    static constexpr int kPageVecs = kF8PageBytes / 16;
+    struct Pair {
+        u32x4 ka[2], kb[2], va[2], vb[2];
+    };
+    static __device__ __forceinline__ void load(Pair &r, const u32x4 *kp, const u32x4 *vp, size_t oa, size_t ob) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            r.ka[h] = __builtin_nontemporal_load(kp + oa + h * 64);
+            r.kb[h] = __builtin_nontemporal_load(kp + ob + h * 64);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            r.va[h] = __builtin_nontemporal_load(vp + oa + h * 64);
+            r.vb[h] = __builtin_nontemporal_load(vp + ob + h * 64);
+        }
+    }
+    template <int PARTS>
+    static __device__ __forceinline__ void consume(Acc &acc, Pair &r, const PairScales &s, const u32x4 (&qop)[4],
+                                                   int first_key, int pos, int ctx, bool hasB, int grp,
+                                                   float scale_log2) {
+        PagePair w;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            widenHalf(w.ka[2 * h], w.ka[2 * h + 1], r.ka[h], s.ka);
+            widenHalf(w.kb[2 * h], w.kb[2 * h + 1], r.kb[h], s.kb);
+            widenHalf(w.va[2 * h], w.va[2 * h + 1], r.va[h], s.va);
+            widenHalf(w.vb[2 * h], w.vb[2 * h + 1], r.vb[h], s.vb);
+        }
+        consumePair<PARTS>(acc, w, qop, first_key, pos, ctx, hasB, grp, scale_log2);
+    }
+};
+// The scales of a lane's page pairs (8-bit pages), and of one of them.
+struct LaneScales {
+    float ka = 0.f, kb = 0.f, va = 0.f, vb = 0.f;
+    __device__ __forceinline__ void load(const float *k_scale, const float *v_scale, int bidA, int bidB, int num_blocks,
+                                         int nkvh, int h) {
+        const int a = unsigned(bidA) < unsigned(num_blocks) ? bidA : 0, b = unsigned(bidB) < unsigned(num_blocks) ? bidB : 0;
+        const size_t ua = size_t(a) * nkvh + h, ub = size_t(b) * nkvh + h;
+        ka = k_scale[ua];
+        kb = k_scale[ub];
+        va = v_scale[ua];
+        vb = v_scale[ub];
+    }
+    __device__ __forceinline__ PairScales of(int lane) const {
+        auto at = [&](float x) {
+            return __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(x)), lane)));
+        };
+        return {at(ka), at(kb), at(va), at(vb)};
+    }
+};
 
 // Output dims of lane (n, grp) for block i: 16*i + 4*grp + {0..3}.
 template <bool OUT_F32>

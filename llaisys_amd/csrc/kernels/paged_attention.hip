@@ -58,8 +58,9 @@ constexpr int kQueueSplitWord = kPrefillQueueWords - 1; // a cache line past the
 struct Args {
     const uint16_t *q;
     void *out;
-    const uint16_t *k_pool;
+    const uint16_t *k_pool; // (8-bit pages: bytes)
     const uint16_t *v_pool;
+    const float *k_scale, *v_scale; // 8-bit pages: per (block, kv head)
     const int32_t *table;
     const int32_t *ctx;
     const int32_t *cu_q;
@@ -167,7 +168,7 @@ typedef u32x4 StageBuf[2][kStagePairs * 16 * 64]; // page pairs: K a, K b, V a, 
 // (groups block * kWaves .. + kWaves - 1 of its groups_b; group_base groups
 // before the sequence), pages [split * pps, ...) of its t.npages. Called by
 // every wave of the workgroup with the same arguments (it has barriers).
-template <bool OUT_F32, bool CHOOSE>
+template <bool OUT_F32, bool CHOOSE, class KV>
 __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b, int block, int group_base, int h,
                                             int split, int pps, int groups_b, const TileGeom &t) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); // uniform: scalar branches on it
@@ -210,6 +211,19 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
         const int i = page - p0;
         return i < 64 ? __builtin_amdgcn_readlane(bid[0], i) : __builtin_amdgcn_readlane(bid[1], i - 64);
     };
+    // 8-bit pages: their scales the same way, of the pool that this wave stages.
+    float scales[2] = {0.f, 0.f};
+    if constexpr (KV::kScaled) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+            if (unsigned(bid[w]) < unsigned(a.num_blocks))
+                scales[w] = ((wave >> 1) & 2 ? a.v_scale : a.k_scale)[size_t(bid[w]) * a.nkvh + h];
+    }
+    auto scaleOf = [&](int page) {
+        const int i = page - p0;
+        return __uint_as_float(uint32_t(i < 64 ? __builtin_amdgcn_readlane(int(__float_as_uint(scales[0])), i)
+                                               : __builtin_amdgcn_readlane(int(__float_as_uint(scales[1])), i - 64)));
+    };
 
     u32x4 qop[kTiles][4];
 #pragma unroll
@@ -231,8 +245,11 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     // Clamped: past the end it re-reads the last pair, so loads are never
     // conditional.
     static_assert(16 % kWaves == 0, "the 16 quarters of a pair split evenly over the waves");
-    constexpr int kPer = 16 / kWaves;
+    // (8-bit pages: 8 one-KiB halves, one per wave: part wave / 2, half wave % 2.)
+    static_assert(!KV::kScaled || kWaves == 8, "one half of an 8-bit page pair per wave");
+    constexpr int kPer = KV::kScaled ? 1 : 16 / kWaves;
     u32x4 st[kStagePairs][kPer];
+    float st_scale[kStagePairs];
     auto stageLoad = [&](int pp) { // the kStagePairs pairs from page pp
 #pragma unroll
         for (int sp = 0; sp < kStagePairs; ++sp) {
@@ -243,7 +260,12 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
             bad_block |= bad;
             ba = bad ? 0 : ba;
             bb = bad ? 0 : bb;
-            const size_t oa = (size_t(ba) * a.nkvh + h) * 256, ob = (size_t(bb) * a.nkvh + h) * 256;
+            const size_t oa = (size_t(ba) * a.nkvh + h) * KV::kPageVecs, ob = (size_t(bb) * a.nkvh + h) * KV::kPageVecs;
+            if constexpr (KV::kScaled) {
+                const int part = wave >> 1, half = wave & 1;
+                st[sp][0] = __builtin_nontemporal_load(((part & 2) ? vp : kp) + ((part & 1) ? ob : oa) + half * 64);
+                st_scale[sp] = scaleOf((part & 1) && q0 + 1 < p1 ? q0 + 1 : q0);
+            } else
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
                 const int q = wave + kWaves * j, part = q >> 2, quarter = q & 3;
@@ -256,21 +278,32 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     // slot (8 + 2 s + h) of a pair holds, per lane, half h (dwords 2h, 2h+1)
     // of V page A's quarter s in its low 8 bytes and of page B's in its high 8.
     auto stageStore = [&](int buf) {
+        auto put = [&](u32x4 *pair, int part, int quarter, u32x4 v) {
+            if (part < 2) {
+                pair[(4 * part + quarter) * 64 + lane] = v;
+            } else {
+                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                u32x2 *half = reinterpret_cast<u32x2 *>(pair + (8 + 2 * quarter) * 64 + lane) + (part & 1);
+                half[0] = u32x2{v[0], v[1]};
+                half[64 * 2] = u32x2{v[2], v[3]}; // next slot, same lane
+            }
+        };
 #pragma unroll
-        for (int sp = 0; sp < kStagePairs; ++sp)
+        for (int sp = 0; sp < kStagePairs; ++sp) {
+            u32x4 *pair = kvs[buf] + sp * 16 * 64;
+            if constexpr (KV::kScaled) { // widened on the way, so the rest of the loop is the bf16 pages'
+                u32x4 q0, q1;
+                widenHalf(q0, q1, st[sp][0], st_scale[sp]);
+                put(pair, wave >> 1, 2 * (wave & 1), q0);
+                put(pair, wave >> 1, 2 * (wave & 1) + 1, q1);
+            } else {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int q = wave + kWaves * j, part = q >> 2, quarter = q & 3;
-                u32x4 *pair = kvs[buf] + sp * 16 * 64;
-                if (part < 2) {
-                    pair[q * 64 + lane] = st[sp][j];
-                } else {
-                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                    u32x2 *half = reinterpret_cast<u32x2 *>(pair + (8 + 2 * quarter) * 64 + lane) + (part & 1);
-                    half[0] = u32x2{st[sp][j][0], st[sp][j][1]};
-                    half[64 * 2] = u32x2{st[sp][j][2], st[sp][j][3]}; // next slot, same lane
+                for (int j = 0; j < kPer; ++j) {
+                    const int q = wave + kWaves * j;
+                    put(pair, q >> 2, q & 3, st[sp][j]);
                 }
             }
+        }
     };
 
     Acc acc[kTiles];
@@ -375,7 +408,7 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     }
 }
 
-template <bool OUT_F32>
+template <bool OUT_F32, class KV>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) prefillKernel(Args a) {
     __shared__ StageBuf kvs;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -395,7 +428,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     t.Lq = __builtin_amdgcn_readfirstlane(t.Lq);
     t.ctx = __builtin_amdgcn_readfirstlane(t.ctx);
     t.npages = __builtin_amdgcn_readfirstlane(t.npages);
-    prefillItem<OUT_F32, false>(a, kvs, b, block, group_base, h, split, a.pps, __builtin_amdgcn_readfirstlane(groupsOf(a, b)),
+    prefillItem<OUT_F32, false, KV>(a, kvs, b, block, group_base, h, split, a.pps, __builtin_amdgcn_readfirstlane(groupsOf(a, b)),
                          t);
 }
 
@@ -406,7 +439,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 // during this item); wave 0 writes the row. The decode kernel's math with
 // kWaves partial states instead of per-wave records.
 constexpr int kDecWindow = 64; // pairs per block-id window (one per lane)
-template <bool OUT_F32>
+template <bool OUT_F32, class KV>
 __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, int h, int row, int c) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
@@ -438,7 +471,9 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
                 bidA = trow[pa];
                 bidB = trow[min(pa + 1, np - 1)];
             }
-            PagePair ring[2];
+            LaneScales scales;
+            if constexpr (KV::kScaled) scales.load(a.k_scale, a.v_scale, bidA, bidB, a.num_blocks, a.nkvh, h);
+            typename KV::Pair ring[2];
             auto issue = [&](int st, int k) {
                 const int kk = min(k, cnt - 1);
                 int bA = __builtin_amdgcn_readlane(bidA, kk);
@@ -447,7 +482,8 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
                 bad_block |= bad;
                 bA = bad ? 0 : bA;
                 bB = bad ? 0 : bB;
-                loadPair(ring[st], kp, vp, (size_t(bA) * a.nkvh + h) * 256, (size_t(bB) * a.nkvh + h) * 256);
+                KV::load(ring[st], kp, vp, (size_t(bA) * a.nkvh + h) * KV::kPageVecs,
+                         (size_t(bB) * a.nkvh + h) * KV::kPageVecs);
             };
             issue(0, 0);
             issue(1, 1);
@@ -457,7 +493,10 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
                     const int k = k0 + st;
                     if (k < cnt) {
                         const int j = base + k;
-                        consumePair<decodeParts<OUT_F32>()>(acc, ring[st], qop, 32 * j, c - 1, c, 2 * j + 1 < np, grp, a.scale_log2);
+                        PairScales ps{};
+                        if constexpr (KV::kScaled) ps = scales.of(k);
+                        KV::template consume<decodeParts<OUT_F32>()>(acc, ring[st], ps, qop, 32 * j, c - 1, c,
+                                                                     2 * j + 1 < np, grp, a.scale_log2);
                     }
                     issue(st, k + 2);
                 }
@@ -570,7 +609,7 @@ __host__ __device__ constexpr size_t queueTableInts(int B, int units) {
     return size_t(6) * (B + 1) + size_t(4) * (units + 1);
 }
 
-template <bool OUT_F32, bool WITH_DECODE, bool CHOOSE>
+template <bool OUT_F32, bool WITH_DECODE, bool CHOOSE, class KV>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
     prefillQueueKernel(Args a) {
     __shared__ StageBuf kvs;
@@ -750,12 +789,12 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             t.nsplit = __builtin_amdgcn_readfirstlane(nspl[u]);
             const int group_base = __builtin_amdgcn_readfirstlane(gbase[b]);
             const int groups_b = __builtin_amdgcn_readfirstlane(gbase[b + 1]) - group_base;
-            prefillItem<OUT_F32, CHOOSE>(a, kvs, b, block, group_base, h, split, pps, groups_b, t);
+            prefillItem<OUT_F32, CHOOSE, KV>(a, kvs, b, block, group_base, h, split, pps, groups_b, t);
         } else if constexpr (WITH_DECODE) {
             const int d = item - n_full;
             const int b = __builtin_amdgcn_readfirstlane(dseq[d / a.nkvh]);
             const int h = d - (d / a.nkvh) * a.nkvh;
-            decodeItem<OUT_F32>(a, kvs, b, h, __builtin_amdgcn_readfirstlane(cu[b]),
+            decodeItem<OUT_F32, KV>(a, kvs, b, h, __builtin_amdgcn_readfirstlane(cu[b]),
                                 __builtin_amdgcn_readfirstlane(ctx[b]));
         }
     }
@@ -929,9 +968,11 @@ bool prefillTakesDecode(int B, int T, const PagedAttentionPlan &plan, const int 
 void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
                   const int32_t *block_table, const int32_t *ctx_len, const int32_t *cu_q, int B, int T, int nh,
                   int nkvh, int max_pages, int num_blocks, float scale, const PagedAttentionPlan &plan,
-                  float *records, int *err, int *queue, void *stream) {
+                  float *records, int *err, int *queue, void *stream, const float *k_scale, const float *v_scale) {
     if (B == 0 || T == 0) return;
     Args a;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
     a.q = q;
     a.out = out;
     a.k_pool = k_pool;
@@ -968,14 +1009,22 @@ void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_
     a.cus = cuCount();
     const dim3 qgrid(unsigned(std::min<long long>(cuCount(), (long long)plan.block_units * a.max_splits)));
     const bool choose = a.pps_min < a.pps;
+    auto launchOver = [&](auto f32, auto chosen, auto kv) {
+        constexpr bool F32 = decltype(f32)::value, CHOOSE = decltype(chosen)::value;
+        using KV = decltype(kv);
+        if (queued && a.with_decode)
+            hipLaunchKernelGGL((prefillQueueKernel<F32, true, CHOOSE, KV>), qgrid, block, unsigned(table_bytes), s, a);
+        else if (queued)
+            hipLaunchKernelGGL((prefillQueueKernel<F32, false, CHOOSE, KV>), qgrid, block, unsigned(table_bytes), s, a);
+        else
+            hipLaunchKernelGGL((prefillKernel<F32, KV>), grid, block, 0, s, a);
+    };
     auto launch = [&](auto f32, auto chosen) {
         constexpr bool F32 = decltype(f32)::value, CHOOSE = decltype(chosen)::value;
-        if (queued && a.with_decode)
-            hipLaunchKernelGGL((prefillQueueKernel<F32, true, CHOOSE>), qgrid, block, unsigned(table_bytes), s, a);
-        else if (queued)
-            hipLaunchKernelGGL((prefillQueueKernel<F32, false, CHOOSE>), qgrid, block, unsigned(table_bytes), s, a);
+        if (k_scale)
+            launchOver(f32, chosen, KvF8());
         else
-            hipLaunchKernelGGL((prefillKernel<F32>), grid, block, 0, s, a);
+            launchOver(f32, chosen, KvBf16());
         if (a.max_splits > 1)
             hipLaunchKernelGGL((prefillCombineKernel<F32, CHOOSE>), dim3(plan.units * kTiles), cblock, 0, s, a);
     };

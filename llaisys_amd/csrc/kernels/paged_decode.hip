@@ -64,8 +64,9 @@ constexpr int kFewUnits = 64;
 struct DecodeArgs {
     const uint16_t *q;
     void *out;
-    const uint16_t *k_pool;
+    const uint16_t *k_pool; // (8-bit pages: bytes)
     const uint16_t *v_pool;
+    const float *k_scale, *v_scale; // 8-bit pages: per (block, kv head)
     const int32_t *table;
     const int32_t *ctx;
     const int32_t *cu_q; // null: query row b is sequence b; else row cu_q[b], and only
@@ -174,8 +175,8 @@ __device__ __forceinline__ float *recordAt(const DecodeArgs &a, int r) {
 __device__ __forceinline__ int recordO(int G, int blk, int col, int grp) { return (blk * G + col) * 16 + grp * 4; }
 __device__ __forceinline__ int recordML(int G, int col) { return G * kHeadDim + 2 * col; }
 
-template <int NSTAGE> struct Ring {
-    PagePair pp[NSTAGE];
+template <int NSTAGE, class KV> struct Ring {
+    typename KV::Pair pp[NSTAGE];
     u32x4 q[NSTAGE][4];
 };
 
@@ -183,7 +184,7 @@ template <int NSTAGE> struct Ring {
 // register file (one wave per SIMD) to avoid spilling. PACKED (bf16): rows
 // go to a.out_packed; a separate instance, since the branch in the finish
 // cost the plain kernel 14 % (53.8 -> 61.3 us at config 3).
-template <bool OUT_F32, int NSTAGE, bool FEW, bool PACKED = false>
+template <bool OUT_F32, int NSTAGE, bool FEW, bool PACKED = false, class KV = KvBf16>
 __global__ void __launch_bounds__(64)
     __attribute__((amdgpu_waves_per_eu(NSTAGE == 2 ? 2 : 1, NSTAGE == 2 ? 2 : 1))) decodeKernel(DecodeArgs a) {
     extern __shared__ int lds[];
@@ -234,6 +235,8 @@ __global__ void __launch_bounds__(64)
         bidA = row[pa];
         bidB = row[pb];
     }
+    LaneScales scales;
+    if constexpr (KV::kScaled) scales.load(a.k_scale, a.v_scale, bidA, bidB, a.num_blocks, a.nkvh, lh);
 
     // Record slot of this wave in its split units (set after the first issues).
     int slot_k[2] = {0, 0}, slot_n[2] = {0, 0};
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(64)
     const u32x4 *vp = reinterpret_cast<const u32x4 *>(a.v_pool) + lane;
     const int ncol = min(n, G - 1); // columns past G read a valid row and are masked later
 
-    Ring<NSTAGE> ring;
+    Ring<NSTAGE, KV> ring;
     bool bad_block = false;
     // Pair k of the window into ring slot st; past the end it re-reads the
     // last pair (an L2 hit), so loads are never conditional and the compiler
@@ -256,7 +259,8 @@ __global__ void __launch_bounds__(64)
         bB = bad ? 0 : bB;
         const int b = __builtin_amdgcn_readlane(lb, kk);
         const int h = __builtin_amdgcn_readlane(lh, kk);
-        loadPair(ring.pp[st], kp, vp, (size_t(bA) * a.nkvh + h) * 256, (size_t(bB) * a.nkvh + h) * 256);
+        KV::load(ring.pp[st], kp, vp, (size_t(bA) * a.nkvh + h) * KV::kPageVecs,
+                 (size_t(bB) * a.nkvh + h) * KV::kPageVecs);
         const uint16_t *qrow = a.q + (size_t(Q[b]) * a.nh + h * G + ncol) * kHeadDim + grp * 8;
 #pragma unroll
         for (int t = 0; t < 4; ++t) ring.q[st][t] = *reinterpret_cast<const u32x4 *>(qrow + 32 * t);
@@ -353,7 +357,10 @@ __global__ void __launch_bounds__(64)
                 u32x4 qop[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) qop[t] = n < G ? ring.q[st][t] : u32x4{0, 0, 0, 0};
-                consumePair<decodeParts<OUT_F32>() - (FEW ? 0 : 1)>(acc, ring.pp[st], qop, 32 * j, c - 1, c, hasB, grp, a.scale_log2);
+                PairScales ps{};
+                if constexpr (KV::kScaled) ps = scales.of(k);
+                KV::template consume<decodeParts<OUT_F32>() - (FEW || KV::kScaled ? 0 : 1)>(acc, ring.pp[st], ps, qop, 32 * j, c - 1, c,
+                                                                             hasB, grp, a.scale_log2);
             }
             issue(st, k + NSTAGE);
         }
@@ -599,7 +606,7 @@ struct RopeArgs {
     bool keep_invalid;  // an invalid length leaves its output rows alone (else zeros)
 };
 
-template <bool OUT_F32, int NSTAGE, bool ROPE>
+template <bool OUT_F32, int NSTAGE, bool ROPE, class KV = KvBf16>
 __global__ void __launch_bounds__(64 * kUnitWaves)
     __attribute__((amdgpu_waves_per_eu(NSTAGE == 2 ? 2 : 1, NSTAGE == 2 ? 2 : 1)))
         decodeUnitKernel(DecodeArgs a, RopeArgs r) {
@@ -672,7 +679,9 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     const u32x4 *kp = reinterpret_cast<const u32x4 *>(a.k_pool) + lane;
     const u32x4 *vp = reinterpret_cast<const u32x4 *>(a.v_pool) + lane;
 
-    PagePair ring[NSTAGE];
+    static_assert(!ROPE || !KV::kScaled, "the fused epilogue writes bf16 pages");
+    typename KV::Pair ring[NSTAGE];
+    LaneScales scales;
     // Pair k of the window into ring slot st (past the window's end its last
     // pair again, an L2 hit, so loads are never conditional).
     auto issue = [&](int st, int k) {
@@ -684,7 +693,8 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
         bad_block |= bad && cnt > 0; // a wave with no pairs loads a stand-in
         bA = bad ? 0 : bA;
         bB = bad ? 0 : bB;
-        loadPair(ring[st], kp, vp, (size_t(bA) * a.nkvh + h) * 256, (size_t(bB) * a.nkvh + h) * 256);
+        KV::load(ring[st], kp, vp, (size_t(bA) * a.nkvh + h) * KV::kPageVecs,
+                 (size_t(bB) * a.nkvh + h) * KV::kPageVecs);
     };
 
     u32x4 qop[4];
@@ -768,6 +778,7 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     for (; base < nw; base += kPairsPerWave) {
         cnt = min(kPairsPerWave, nw - base);
         if (base != 0) loadWindow();
+        if constexpr (KV::kScaled) scales.load(a.k_scale, a.v_scale, bidA, bidB, a.num_blocks, a.nkvh, h);
         if (!issued) {
 #pragma unroll
             for (int st = 0; st < NSTAGE; ++st) issue(st, st);
@@ -782,7 +793,10 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
                 const int k = k0 + st;
                 if (k < cnt_c) {
                     const int j = wave + kUnitWaves * (base + k);
-                    consumePair<decodeParts<OUT_F32>()>(acc, ring[st], qop, 32 * j, c - 1, c, 2 * j + 1 < np, grp, a.scale_log2);
+                    PairScales ps{};
+                    if constexpr (KV::kScaled) ps = scales.of(k);
+                    KV::template consume<decodeParts<OUT_F32>()>(acc, ring[st], ps, qop, 32 * j, c - 1, c,
+                                                                 2 * j + 1 < np, grp, a.scale_log2);
                 }
                 issue(st, k + NSTAGE);
             }
@@ -938,7 +952,7 @@ void pagedDecodeNoAlloc(void *out, bool out_f32, const uint16_t *q, const uint16
     // chunks run one after another on the stream and reuse the records.
     for (int b0 = 0; b0 < B; b0 += kDecodeMaxBatch) {
         const int Bc = std::min(kDecodeMaxBatch, B - b0);
-        DecodePlan plan = planDecode(Bc, nkvh, G, max_pages);
+        DecodePlan plan = planDecode(Bc, nkvh, G, max_pages, false);
         plan.slot_headers = 0; // per-wave records only: nothing to keep zeroed between calls
         plan.slot_record_bytes = 0;
         LLAISYS_CHECK(plan.record_bytes <= kNoAllocScratchBytes,
@@ -962,14 +976,14 @@ namespace {
 int slotsFor(int B, int nkvh) { return (long long)B * nkvh <= kManySlotUnits ? kManySlots : kFirstSlots; }
 } // namespace
 
-DecodePlan planDecode(int B, int nkvh, int group, int max_pages) {
+DecodePlan planDecode(int B, int nkvh, int group, int max_pages, bool f8) {
     DecodePlan p{};
     const long long max_pairs = (long long)B * nkvh * ((max_pages + 1) / 2);
     // 1.75 waves per CU: measured best for the model's 128 x ~2100-token
     // batches (3.54 ms per step against 3.56-3.60 at 1.5 and 3.56 at 2 waves
     // per CU; 1 wave per CU was 3 % slower than 1.5), slightly ahead for the
     // mixed batch and neutral for the config-3 batch (53.15 us at 1.5 or 1.75).
-    const int fill = std::max(1, envInt("LLAISYS_DECODE_WAVES", computeUnits() * 7 / 4));
+    const int fill = std::max(1, envInt("LLAISYS_DECODE_WAVES", f8 ? computeUnits() * 4 : computeUnits() * 7 / 4));
     p.waves = int(std::max<long long>(fill, (max_pairs + kPairsPerWave - 1) / kPairsPerWave));
     p.record_bytes = size_t(2) * p.waves * group * (kHeadDim + 2) * sizeof(float);
     p.lds_bytes = size_t(3 * B + 1) * sizeof(int);
@@ -987,9 +1001,12 @@ void pagedDecode(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_p
                  const int32_t *block_table, const int32_t *ctx_len, const int32_t *cu_q, int B, int T, int nh,
                  int nkvh, int max_pages,
                  int num_blocks, float scale, const DecodePlan &plan, float *records, int *err,
-                 int *slot_headers, void *slot_records, void *stream, uint16_t *out_packed) {
+                 int *slot_headers, void *slot_records, void *stream, uint16_t *out_packed, const float *k_scale,
+                 const float *v_scale) {
     if (B == 0) return;
     DecodeArgs a;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
     a.q = q;
     a.out = out;
     a.k_pool = k_pool;
@@ -1021,7 +1038,9 @@ void pagedDecode(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_p
     const dim3 grid(plan.waves), block(64), comb(B * nkvh), comb_block(64 * kCombineWaves);
     auto launch = [&](auto f32, auto few, auto packed) {
         constexpr bool F32 = decltype(f32)::value, FEW = decltype(few)::value, PACKED = decltype(packed)::value;
-        if (plan.stages == 3)
+        if (k_scale) {
+            if constexpr (!PACKED) hipLaunchKernelGGL((decodeKernel<F32, 2, FEW, false, KvF8>), grid, block, lds, s, a);
+        } else if (plan.stages == 3)
             hipLaunchKernelGGL((decodeKernel<F32, 3, FEW, PACKED>), grid, block, lds, s, a);
         else
             hipLaunchKernelGGL((decodeKernel<F32, 2, FEW, PACKED>), grid, block, lds, s, a);
@@ -1029,6 +1048,7 @@ void pagedDecode(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_p
     };
     const std::true_type yes;
     const std::false_type no;
+    LLAISYS_CHECK(!k_scale || !out_packed, "pagedDecode: 8-bit pages have no packed output");
     if (out_f32)
         a.few ? launch(yes, yes, no) : launch(yes, no, no);
     else if (out_packed)
@@ -1041,9 +1061,12 @@ void pagedDecode(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_p
 namespace {
 void launchDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
                        const int32_t *block_table, const int32_t *ctx_len, int B, int nh, int nkvh, int max_pages,
-                       int num_blocks, float scale, int *err, const RopeArgs &r, bool rope, void *stream) {
+                       int num_blocks, float scale, int *err, const RopeArgs &r, bool rope, void *stream,
+                       const float *k_scale = nullptr, const float *v_scale = nullptr) {
     if (B == 0) return;
     DecodeArgs a{};
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
     a.q = q;
     a.out = out;
     a.k_pool = k_pool;
@@ -1062,7 +1085,12 @@ void launchDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_
     // Two page pairs in flight per wave (see kUnitWaves for the measurements).
     auto s = static_cast<hipStream_t>(stream);
     const dim3 grid(unsigned(B) * unsigned(nkvh)), block(64 * kUnitWaves);
-    if (rope) {
+    if (k_scale) {
+        if (out_f32)
+            hipLaunchKernelGGL((decodeUnitKernel<true, 2, false, KvF8>), grid, block, 0, s, a, r);
+        else
+            hipLaunchKernelGGL((decodeUnitKernel<false, 2, false, KvF8>), grid, block, 0, s, a, r);
+    } else if (rope) {
         if (out_f32)
             hipLaunchKernelGGL((decodeUnitKernel<true, 2, true>), grid, block, 0, s, a, r);
         else
@@ -1079,14 +1107,15 @@ void launchDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_
 
 void pagedDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
                       const int32_t *block_table, const int32_t *ctx_len, int B, int nh, int nkvh, int max_pages,
-                      int num_blocks, float scale, int *err, void *stream, uint16_t *out_packed, bool keep_invalid) {
+                      int num_blocks, float scale, int *err, void *stream, uint16_t *out_packed, bool keep_invalid,
+                      const float *k_scale, const float *v_scale) {
     LLAISYS_CHECK(!out_packed || (!out_f32 && (nh * kHeadDim) % 32 == 0),
                   "pagedDecodeUnits: a packed output is bf16 with nh * 128 % 32 == 0");
     RopeArgs r{};
     r.o_packed = out_packed;
     r.keep_invalid = keep_invalid;
     launchDecodeUnits(out, out_f32, q, k_pool, v_pool, block_table, ctx_len, B, nh, nkvh, max_pages, num_blocks,
-                      scale, err, r, false, stream);
+                      scale, err, r, false, stream, k_scale, v_scale);
 }
 
 bool decodeUnitsRopeSupported(int nh, int nkvh, int d) {

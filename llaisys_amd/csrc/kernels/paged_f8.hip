@@ -1,11 +1,9 @@
-// Append, gather and block copy of the 8-bit paged KV, and attention over it
-// (f8_page.hpp has the format).
+// Append, gather and block copy of the 8-bit paged KV (f8_page.hpp has the
+// format).
 #include "f8_page.hpp"
 #include "mfma_common.hpp"
 
 #include "../device/hip_check.hpp"
-
-#include <type_traits>
 
 namespace llaisys::kernels {
 
@@ -151,12 +149,6 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------- gather
 
-// Two of a word's four codes (the high two if `hi`) as bf16, times the scale;
-// exact (4 significant bits).
-template <bool HI> __device__ __forceinline__ uint32_t widen2(uint32_t w, float scale) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
-}
-
 // One 256-thread workgroup per (page, sequence, kv head): the pages go through
 // LDS as bf16 rows and out row by row.
 __global__ void __launch_bounds__(256)
@@ -229,88 +221,6 @@ __global__ void __launch_bounds__(256)
     for (int h = threadIdx.x; h < nkvh; h += 256) scale[size_t(dst) * nkvh + h] = scale[size_t(src) * nkvh + h];
 }
 
-// --------------------------------------------------------------- attention
-
-// One wave per (query row, kv head): the row's keys, a page pair at a time.
-template <bool OUT_F32>
-__global__ void __launch_bounds__(64)
-    attentionF8Kernel(void *out, const uint16_t *__restrict__ q, const uint8_t *__restrict__ k_pool,
-                      const uint8_t *__restrict__ v_pool, const float *__restrict__ k_scale,
-                      const float *__restrict__ v_scale, const int32_t *__restrict__ table,
-                      const int32_t *__restrict__ ctx, const int32_t *__restrict__ cu_q, int B, int T, int nh,
-                      int nkvh, int max_pages, int num_blocks, float scale_log2, int *err) {
-    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, n = lane & 15, grp = lane >> 4;
-    const int G = nh / nkvh;
-    int b = row, lq = 1, qi = 0;
-    if (cu_q) {
-        int lo = 0, hi = B - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (cu_q[mid] <= row)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        b = lo;
-        qi = row - cu_q[b];
-        lq = cu_q[b + 1] - cu_q[b];
-        if (qi < 0 || qi >= lq) return; // before the first or behind the last sequence
-    }
-    const int c = ctx[b];
-    if (c < lq || c > max_pages * 16) {
-        if (lane == 0) atomicOr(err, kErrTooLong);
-        return;
-    }
-    const int keys = c - lq + qi + 1;
-    u32x4 qop[4];
-    const uint16_t *qrow = q + (size_t(row) * nh + h * G + min(n, G - 1)) * kHeadDim + grp * 8;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        qop[s] = *reinterpret_cast<const u32x4 *>(qrow + 32 * s);
-        qop[s] = n < G ? qop[s] : u32x4{0, 0, 0, 0};
-    }
-    Acc acc;
-    acc.reset();
-    bool bad = false;
-    const int np = (keys + 15) >> 4;
-    for (int p = 0; p < np; p += 2) {
-        PagePair pair;
-        auto page = [&](int at, u32x4 (&k)[4], u32x4 (&v)[4]) {
-            int blk = table[size_t(b) * max_pages + at];
-            if (unsigned(blk) >= unsigned(num_blocks)) {
-                bad = true;
-                blk = 0;
-            }
-            const size_t unit = size_t(blk) * nkvh + h;
-            const float ks = k_scale[unit], vs = v_scale[unit];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const u32x4 kc = reinterpret_cast<const u32x4 *>(k_pool + unit * kF8PageBytes)[64 * half + lane];
-                const u32x4 vc = reinterpret_cast<const u32x4 *>(v_pool + unit * kF8PageBytes)[64 * half + lane];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    k[2 * half + j] = u32x4{widen2<false>(kc[2 * j], ks), widen2<true>(kc[2 * j], ks),
-                                            widen2<false>(kc[2 * j + 1], ks), widen2<true>(kc[2 * j + 1], ks)};
-                    v[2 * half + j] = u32x4{widen2<false>(vc[2 * j], vs), widen2<true>(vc[2 * j], vs),
-                                            widen2<false>(vc[2 * j + 1], vs), widen2<true>(vc[2 * j + 1], vs)};
-                }
-            }
-        };
-        const bool hasB = p + 1 < np;
-        page(p, pair.ka, pair.va);
-        page(hasB ? p + 1 : p, pair.kb, pair.vb);
-        consumePair<decodeParts<OUT_F32>()>(acc, pair, qop, 16 * p, keys - 1, keys, hasB, grp, scale_log2);
-    }
-    if (bad && lane == 0) atomicOr(err, kErrBadBlock);
-    float l = acc.l + __shfl_xor(acc.l, 16);
-    l += __shfl_xor(l, 32);
-    if (n >= G) return;
-    const float inv = 1.f / l;
-    const size_t orow = (size_t(row) * nh + h * G + n) * kHeadDim;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) storeOut<OUT_F32>(out, orow, i, grp, acc.o[i] * inv);
-}
-
 } // namespace
 
 void pagedAppendF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale, const uint16_t *k_new,
@@ -338,23 +248,6 @@ void pagedCopyBlocksF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *
     if (P == 0) return;
     hipLaunchKernelGGL(copyBlocksF8Kernel, dim3(unsigned(P), 2), dim3(256), 0, static_cast<hipStream_t>(stream),
                        k_pool, v_pool, k_scale, v_scale, pairs, nkvh, num_blocks, err);
-    HIP_CHECK(hipGetLastError());
-}
-
-void pagedAttentionF8(void *out, bool out_f32, const uint16_t *q, const uint8_t *k_pool, const uint8_t *v_pool,
-                      const float *k_scale, const float *v_scale, const int32_t *block_table, const int32_t *ctx_len,
-                      const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
-                      int *err, void *stream) {
-    if (B == 0 || T == 0) return;
-    auto launch = [&](auto f32) {
-        hipLaunchKernelGGL(attentionF8Kernel<decltype(f32)::value>, dim3(unsigned(T), unsigned(nkvh)), dim3(64), 0,
-                           static_cast<hipStream_t>(stream), out, q, k_pool, v_pool, k_scale, v_scale, block_table,
-                           ctx_len, cu_q, B, T, nh, nkvh, max_pages, num_blocks, scale * 1.4426950408889634f, err);
-    };
-    if (out_f32)
-        launch(std::true_type());
-    else
-        launch(std::false_type());
     HIP_CHECK(hipGetLastError());
 }
 

@@ -5,20 +5,30 @@
 // misses, or leave one that it is; the remainder x - q s decides: it is exact
 // (its bits reach from those of s to half of s), so q is the exact quotient's
 // rounding whatever the division did.
+//
+// A row is read once and its codes written once: a thread keeps its pieces of
+// the row (16 B each) in registers from the search for the largest magnitude
+// to the codes; what goes past kPieces of them is read again, from the caches.
 #include "launch.hpp"
 
 #include "../device/hip_check.hpp"
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 namespace llaisys::kernels {
 
 namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <ElemType T> struct Elem;
 template <> struct Elem<ElemType::BF16> { using type = __bf16; };
 template <> struct Elem<ElemType::F16> { using type = _Float16; };
 template <> struct Elem<ElemType::F32> { using type = float; };
+
+constexpr int kPieces = 5; // of a thread, in registers
 
 // x / s to the nearest whole number (|x| <= 127.5 s, s > 0); inv about 1 / s.
 __device__ __forceinline__ int quantized(float x, float s, float inv) {
@@ -29,51 +39,116 @@ __device__ __forceinline__ int quantized(float x, float s, float inv) {
     return int(fminf(fmaxf(q, -127.f), 127.f));
 }
 
-__device__ __forceinline__ float waveMax(float x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
-    return x;
-}
-
-// One wave per row: its largest magnitude, then its codes.
-template <ElemType T>
-__global__ void __launch_bounds__(256) quantizeRowsKernel(int8_t *__restrict__ q, float *__restrict__ scale,
-                                                          const void *__restrict__ x, int M, int K) {
+// A row by WAVES waves (WAVES == 1: four rows a workgroup). VEC: rows of whole
+// 16 B pieces, aligned; else piece by piece of one element.
+template <ElemType T, int WAVES, bool VEC>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
+    quantizeRowsKernel(int8_t *__restrict__ q, float *__restrict__ scale, const void *__restrict__ x, int M, int K) {
     using E = typename Elem<T>::type;
-    const int lane = threadIdx.x & 63;
-    const int m = int(blockIdx.x) * 4 + int(threadIdx.x >> 6);
+    constexpr int EL = VEC ? 16 / int(sizeof(E)) : 1; // elements of a piece
+    constexpr int THREADS = 64 * WAVES;
+    __shared__ float tops[WAVES];
+    const int tid = WAVES == 1 ? int(threadIdx.x & 63) : int(threadIdx.x);
+    const int m = WAVES == 1 ? int(blockIdx.x) * 4 + int(threadIdx.x >> 6) : int(blockIdx.x);
     if (m >= M) return;
     const E *row = static_cast<const E *>(x) + size_t(m) * K;
     int8_t *to = q + size_t(m) * K;
-    float top = 0.f;
-    bool finite = true;
-    for (int k = lane; k < K; k += 64) {
-        const float v = fabsf(float(row[k]));
-        finite = finite && v < INFINITY;
-        top = fmaxf(top, v);
+    const int pieces = K / EL;
+    struct Piece {
+        E e[EL];
+    };
+    auto load = [&](int p) {
+        Piece r;
+        if constexpr (VEC)
+            r = __builtin_bit_cast(Piece, reinterpret_cast<const u32x4 *>(row)[p]);
+        else
+            r.e[0] = row[p];
+        return r;
+    };
+    // The largest magnitude as bits: they order as the numbers do, and those of
+    // infinities and NaNs come last.
+    uint32_t top = 0;
+    auto search = [&](const Piece &r) {
+#pragma unroll
+        for (int e = 0; e < EL; ++e) top = max(top, __float_as_uint(float(r.e[e])) & 0x7fffffffu);
+    };
+    Piece held[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) held[i] = load(max(0, min(tid + i * THREADS, pieces - 1)));
+    if (pieces > 0) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) search(held[i]);
     }
-    top = waveMax(top);
-    finite = __ballot(!finite) == 0;
-    const float s = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
-    if (lane == 0) scale[m] = s;
+    for (int p = tid + kPieces * THREADS; p < pieces; p += THREADS) search(load(p));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), off)));
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = __uint_as_float(top);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = max(top, __float_as_uint(tops[w]));
+    }
+    const bool finite = top < 0x7f800000u;
+    const float most = __uint_as_float(top);
+    const float s = finite ? most / 127.f : __uint_as_float(0x7fc00000u);
+    if (tid == 0) scale[m] = s;
     // Rows of very small values: the same quotients from larger numbers, whose inverse is finite.
-    const float grow = top < 0x1p-60f ? 0x1p80f : 1.f, sg = s * grow, inv = 1.f / sg;
+    const float grow = most < 0x1p-60f ? 0x1p80f : 1.f, sg = s * grow, inv = 1.f / sg;
     const bool some = finite && s > 0.f;
-    for (int k = lane; k < K; k += 64) to[k] = some ? int8_t(quantized(float(row[k]) * grow, sg, inv)) : int8_t(0);
+    auto store = [&](int p, const Piece &r) {
+        uint32_t w[EL > 4 ? 2 : 1] = {};
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+            const int c = some ? quantized(float(r.e[e]) * grow, sg, inv) : 0;
+            w[e / 4] |= (uint32_t(c) & 0xffu) << (8 * (e & 3));
+        }
+        if constexpr (EL == 8)
+            reinterpret_cast<uint2 *>(to)[p] = make_uint2(w[0], w[1]);
+        else if constexpr (EL == 4)
+            reinterpret_cast<uint32_t *>(to)[p] = w[0];
+        else
+            to[p] = int8_t(w[0]);
+    };
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+        if (tid + i * THREADS < pieces) store(tid + i * THREADS, held[i]);
+    for (int p = tid + kPieces * THREADS; p < pieces; p += THREADS) store(p, load(p));
+}
+
+template <ElemType T, bool VEC>
+void launchQuantize(int8_t *q, float *scale, const void *x, int M, int K, hipStream_t s) {
+    const int pieces = VEC ? K / (16 / int(sizeof(typename Elem<T>::type))) : K;
+    // As many waves as hold the row (1500 x 8960: a wave per row, reading most
+    // of it twice, 14.6 us).
+    if (pieces <= 64 * kPieces)
+        hipLaunchKernelGGL((quantizeRowsKernel<T, 1, VEC>), dim3(unsigned((M + 3) / 4)), dim3(256), 0, s, q, scale, x, M, K);
+    else if (pieces <= 256 * kPieces)
+        hipLaunchKernelGGL((quantizeRowsKernel<T, 4, VEC>), dim3(unsigned(M)), dim3(256), 0, s, q, scale, x, M, K);
+    else
+        hipLaunchKernelGGL((quantizeRowsKernel<T, 16, VEC>), dim3(unsigned(M)), dim3(1024), 0, s, q, scale, x, M, K);
+    HIP_CHECK(hipGetLastError());
+}
+
+template <ElemType T> void quantizeAs(int8_t *q, float *scale, const void *x, int M, int K, hipStream_t s) {
+    constexpr int es = int(sizeof(typename Elem<T>::type));
+    const bool vec = size_t(K) * es % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(q) % (16 / es) == 0;
+    if (vec)
+        launchQuantize<T, true>(q, scale, x, M, K, s);
+    else
+        launchQuantize<T, false>(q, scale, x, M, K, s);
 }
 
 } // namespace
 
 void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K, void *stream) {
     if (M == 0) return;
-    const dim3 grid(unsigned((M + 3) / 4)), block(256);
     auto s = static_cast<hipStream_t>(stream);
     switch (t) {
-    case ElemType::F32: hipLaunchKernelGGL(quantizeRowsKernel<ElemType::F32>, grid, block, 0, s, q, scale, x, M, K); break;
-    case ElemType::F16: hipLaunchKernelGGL(quantizeRowsKernel<ElemType::F16>, grid, block, 0, s, q, scale, x, M, K); break;
-    case ElemType::BF16: hipLaunchKernelGGL(quantizeRowsKernel<ElemType::BF16>, grid, block, 0, s, q, scale, x, M, K); break;
+    case ElemType::F32: quantizeAs<ElemType::F32>(q, scale, x, M, K, s); break;
+    case ElemType::F16: quantizeAs<ElemType::F16>(q, scale, x, M, K, s); break;
+    case ElemType::BF16: quantizeAs<ElemType::BF16>(q, scale, x, M, K, s); break;
     }
-    HIP_CHECK(hipGetLastError());
 }
 
 } // namespace llaisys::kernels

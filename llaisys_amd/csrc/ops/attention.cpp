@@ -317,6 +317,72 @@ AttnDims checkAttention(const char *op, const tensor_t &out, const tensor_t &q, 
 
 } // namespace
 
+namespace {
+
+// The checked call on the device: bf16 pages, or 8-bit ones with their scales.
+void attendOnDevice(const char *op, const tensor_t &out, const tensor_t &q, const tensor_t &k_pool,
+                    const tensor_t &v_pool, const tensor_t &k_scale, const tensor_t &v_scale,
+                    const tensor_t &block_table, const tensor_t &ctx_len, const tensor_t &cu_q, float scale,
+                    bool stream_k) {
+    const size_t T = q->shape()[0], nh = q->shape()[1], nkvh = k_pool->shape()[1], B = ctx_len->shape()[0];
+    const int max_pages = int(block_table->shape()[1]);
+    auto &rt = core::context().runtime();
+    const int G = int(nh / nkvh);
+    const bool f32 = out->dtype() == LLAISYS_DTYPE_F32;
+    const auto *qp = reinterpret_cast<const uint16_t *>(q->data());
+    const auto *kp = reinterpret_cast<const uint16_t *>(k_pool->data());
+    const auto *vp = reinterpret_cast<const uint16_t *>(v_pool->data());
+    const auto *tab = reinterpret_cast<const int32_t *>(block_table->data());
+    const auto *ctx = reinterpret_cast<const int32_t *>(ctx_len->data());
+    const int nb = int(k_pool->shape()[0]);
+    const float *ks = k_scale ? reinterpret_cast<const float *>(k_scale->data()) : nullptr;
+    const float *vs = v_scale ? reinterpret_cast<const float *>(v_scale->data()) : nullptr;
+    if (!cu_q && !stream_k && K::unitDecodeTakes(int(B), int(nkvh), max_pages)) {
+        K::pagedDecodeUnits(out->data(), f32, qp, kp, vp, tab, ctx, int(B), int(nh), int(nkvh), max_pages, nb, scale,
+                            rt.errorWord(), rt.stream(), nullptr, true, ks, vs);
+        return;
+    }
+    if (!cu_q) {
+        // Decode: sequences are independent, so large batches run in chunks
+        // whose length prefix fits the kernel's LDS.
+        for (size_t b0 = 0; b0 < B; b0 += K::kDecodeMaxBatch) {
+            const int Bc = int(std::min<size_t>(K::kDecodeMaxBatch, B - b0));
+            auto plan = K::planDecode(Bc, int(nkvh), G, max_pages, ks != nullptr);
+            float *records = static_cast<float *>(rt.scratch(plan.record_bytes));
+            const size_t esz = f32 ? 4 : 2;
+            K::pagedDecode(static_cast<std::byte *>(out->data()) + b0 * nh * K::kHeadDim * esz, f32,
+                           qp + b0 * nh * K::kHeadDim, kp, vp, tab + b0 * size_t(max_pages), ctx + b0, nullptr, Bc,
+                           Bc, int(nh), int(nkvh), max_pages, nb, scale, plan, records, rt.errorWord(),
+                           plan.slot_headers ? rt.decodeSlotHeaders(plan.slot_headers) : nullptr,
+                           plan.slot_headers ? rt.decodeSlotRecords(plan.slot_record_bytes) : nullptr, rt.stream(),
+                           nullptr, ks, vs);
+        }
+        return;
+    }
+    // Varlen: single-query sequences through the decode kernel, the rest
+    // through the prefill kernel; both read the same cu_q and skip the other's.
+    LLAISYS_CHECK(B <= size_t(K::kDecodeMaxBatch),
+                  op << ": at most " << K::kDecodeMaxBatch << " sequences per varlen call");
+    const auto *cu = reinterpret_cast<const int32_t *>(cu_q->data());
+    auto dplan = K::planDecode(int(B), int(nkvh), G, max_pages, ks != nullptr);
+    auto pplan = K::planPrefill(int(B), int(T), int(nkvh), G, max_pages);
+    float *records = static_cast<float *>(rt.scratch(std::max(dplan.record_bytes, pplan.partial_bytes)));
+    int *queue = rt.queueCounters();
+    // The persistent prefill kernel takes the single-query sequences too
+    // when it runs (their HBM-bound work then overlaps the prefill's MFMA
+    // work); otherwise the decode kernel does.
+    if (!K::prefillTakesDecode(int(B), int(T), pplan, queue)) {
+        int *slot_hdr = dplan.slot_headers ? rt.decodeSlotHeaders(dplan.slot_headers) : nullptr;
+        void *slot_rec = dplan.slot_headers ? rt.decodeSlotRecords(dplan.slot_record_bytes) : nullptr;
+        K::pagedDecode(out->data(), f32, qp, kp, vp, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh), max_pages, nb,
+                       scale, dplan, records, rt.errorWord(), slot_hdr, slot_rec, rt.stream(), nullptr, ks, vs);
+    }
+    K::pagedPrefill(out->data(), f32, qp, kp, vp, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh), max_pages, nb,
+                    scale, pplan, records, rt.errorWord(), queue, rt.stream(), ks, vs);
+}
+
+} // namespace
+
 void pagedAttention(const tensor_t &out, const tensor_t &q, const tensor_t &k_pool, const tensor_t &v_pool,
                     const tensor_t &block_table, const tensor_t &ctx_len, const tensor_t &cu_q, float scale,
                     bool stream_k) {
@@ -335,56 +401,7 @@ void pagedAttention(const tensor_t &out, const tensor_t &q, const tensor_t &k_po
                                  reinterpret_cast<const int32_t *>(ctx_len->data()),
                                  cu_q ? reinterpret_cast<const int32_t *>(cu_q->data()) : nullptr, int(B), int(T),
                                  int(nh), int(nkvh), max_pages, int(k_pool->shape()[0]), scale, errWord());
-    auto &rt = core::context().runtime();
-    const int G = int(nh / nkvh);
-    const bool f32 = out->dtype() == LLAISYS_DTYPE_F32;
-    const auto *qp = reinterpret_cast<const uint16_t *>(q->data());
-    const auto *kp = reinterpret_cast<const uint16_t *>(k_pool->data());
-    const auto *vp = reinterpret_cast<const uint16_t *>(v_pool->data());
-    const auto *tab = reinterpret_cast<const int32_t *>(block_table->data());
-    const auto *ctx = reinterpret_cast<const int32_t *>(ctx_len->data());
-    const int nb = int(k_pool->shape()[0]);
-    if (!cu_q && !stream_k && K::unitDecodeTakes(int(B), int(nkvh), max_pages)) {
-        K::pagedDecodeUnits(out->data(), f32, qp, kp, vp, tab, ctx, int(B), int(nh), int(nkvh), max_pages, nb, scale,
-                            rt.errorWord(), rt.stream(), nullptr, true);
-        return;
-    }
-    if (!cu_q) {
-        // Decode: sequences are independent, so large batches run in chunks
-        // whose length prefix fits the kernel's LDS.
-        for (size_t b0 = 0; b0 < B; b0 += K::kDecodeMaxBatch) {
-            const int Bc = int(std::min<size_t>(K::kDecodeMaxBatch, B - b0));
-            auto plan = K::planDecode(Bc, int(nkvh), G, max_pages);
-            float *records = static_cast<float *>(rt.scratch(plan.record_bytes));
-            const size_t esz = f32 ? 4 : 2;
-            K::pagedDecode(static_cast<std::byte *>(out->data()) + b0 * nh * K::kHeadDim * esz, f32,
-                           qp + b0 * nh * K::kHeadDim, kp, vp, tab + b0 * size_t(max_pages), ctx + b0, nullptr, Bc,
-                           Bc, int(nh), int(nkvh), max_pages, nb, scale, plan, records, rt.errorWord(),
-                           plan.slot_headers ? rt.decodeSlotHeaders(plan.slot_headers) : nullptr,
-                           plan.slot_headers ? rt.decodeSlotRecords(plan.slot_record_bytes) : nullptr, rt.stream());
-        }
-        return;
-    }
-    // Varlen: single-query sequences through the decode kernel, the rest
-    // through the prefill kernel; both read the same cu_q and skip the other's.
-    LLAISYS_CHECK(B <= size_t(K::kDecodeMaxBatch),
-                  op << ": at most " << K::kDecodeMaxBatch << " sequences per varlen call");
-    const auto *cu = reinterpret_cast<const int32_t *>(cu_q->data());
-    auto dplan = K::planDecode(int(B), int(nkvh), G, max_pages);
-    auto pplan = K::planPrefill(int(B), int(T), int(nkvh), G, max_pages);
-    float *records = static_cast<float *>(rt.scratch(std::max(dplan.record_bytes, pplan.partial_bytes)));
-    int *queue = rt.queueCounters();
-    // The persistent prefill kernel takes the single-query sequences too
-    // when it runs (their HBM-bound work then overlaps the prefill's MFMA
-    // work); otherwise the decode kernel does.
-    if (!K::prefillTakesDecode(int(B), int(T), pplan, queue)) {
-        int *slot_hdr = dplan.slot_headers ? rt.decodeSlotHeaders(dplan.slot_headers) : nullptr;
-        void *slot_rec = dplan.slot_headers ? rt.decodeSlotRecords(dplan.slot_record_bytes) : nullptr;
-        K::pagedDecode(out->data(), f32, qp, kp, vp, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh), max_pages, nb,
-                       scale, dplan, records, rt.errorWord(), slot_hdr, slot_rec, rt.stream());
-    }
-    K::pagedPrefill(out->data(), f32, qp, kp, vp, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh), max_pages, nb,
-                    scale, pplan, records, rt.errorWord(), queue, rt.stream());
+    attendOnDevice(op, out, q, k_pool, v_pool, nullptr, nullptr, block_table, ctx_len, cu_q, scale, stream_k);
 }
 
 // No counterpart in the reference: the decode above for callers that cannot
@@ -557,21 +574,18 @@ void pagedAttentionF8(const tensor_t &out, const tensor_t &q, const tensor_t &k_
     if (T == 0 || B == 0) return;
     const int max_pages = int(block_table->shape()[1]);
     LLAISYS_CHECK(max_pages > 0, op << ": block_table has no pages");
-    const bool f32 = out->dtype() == LLAISYS_DTYPE_F32;
-    const auto *qp = reinterpret_cast<const uint16_t *>(q->data());
-    const auto *kp = reinterpret_cast<const uint8_t *>(k_pool->data());
-    const auto *vp = reinterpret_cast<const uint8_t *>(v_pool->data());
-    const auto *ks = reinterpret_cast<const float *>(k_scale->data());
-    const auto *vs = reinterpret_cast<const float *>(v_scale->data());
-    const auto *tab = reinterpret_cast<const int32_t *>(block_table->data());
-    const auto *ctx = reinterpret_cast<const int32_t *>(ctx_len->data());
-    const auto *cu = cu_q ? reinterpret_cast<const int32_t *>(cu_q->data()) : nullptr;
-    const int nb = int(k_pool->shape()[0]);
-    if (host)
-        return C::pagedAttentionF8(out->data(), f32, qp, kp, vp, ks, vs, tab, ctx, cu, int(B), int(T), int(nh),
-                                   int(nkvh), max_pages, nb, scale, errWord());
-    K::pagedAttentionF8(out->data(), f32, qp, kp, vp, ks, vs, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh),
-                        max_pages, nb, scale, errWord(), streamOf());
+    LLAISYS_CHECK(k_pool->shape()[0] > 0, op << ": the pool has no blocks");
+    if (!host)
+        return attendOnDevice(op, out, q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_len, cu_q, scale, false);
+    C::pagedAttentionF8(out->data(), out->dtype() == LLAISYS_DTYPE_F32, reinterpret_cast<const uint16_t *>(q->data()),
+                        reinterpret_cast<const uint8_t *>(k_pool->data()),
+                        reinterpret_cast<const uint8_t *>(v_pool->data()),
+                        reinterpret_cast<const float *>(k_scale->data()),
+                        reinterpret_cast<const float *>(v_scale->data()),
+                        reinterpret_cast<const int32_t *>(block_table->data()),
+                        reinterpret_cast<const int32_t *>(ctx_len->data()),
+                        cu_q ? reinterpret_cast<const int32_t *>(cu_q->data()) : nullptr, int(B), int(T), int(nh),
+                        int(nkvh), max_pages, int(k_pool->shape()[0]), scale, errWord());
 }
 
 } // namespace llaisys::ops
