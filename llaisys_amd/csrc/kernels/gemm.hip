@@ -1229,17 +1229,33 @@ void linear(void *y, const void *x, const void *w, const void *bias, ElemType t,
 
 namespace {
 
-// Rows that are not whole 16 B pieces: one thread per output.
-template <ElemType O>
-__global__ void __launch_bounds__(256) gemmRowsI8Kernel(GemmParams p) {
+// Rows of K bytes, or of whatever alignment, as rows of Kp = whole 16 B pieces
+// with zeros behind: what the tiles and the few-rows kernel read. x and w of a
+// call in one launch, 16 B a thread.
+__global__ void __launch_bounds__(256)
+    padRowsKernel(int8_t *__restrict__ to, const int8_t *__restrict__ x, const int8_t *__restrict__ w, int M, int N, int K,
+                  int Kp) {
+    const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x;
+    const int pieces = Kp / 16;
+    const size_t row = i / pieces;
+    if (row >= size_t(M) + N) return;
+    const int k0 = int(i - row * pieces) * 16;
+    const int8_t *from = row < size_t(M) ? x + row * K : w + (row - M) * K;
+    uint32_t v[4] = {};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const uint32_t b = k0 + e < K ? uint32_t(uint8_t(from[k0 + e])) : 0u;
+        v[e / 4] |= b << (8 * (e & 3));
+    }
+    reinterpret_cast<u32x4 *>(to)[i] = u32x4{v[0], v[1], v[2], v[3]};
+}
+
+// Sums over no products at all (K = 0).
+template <ElemType O> __global__ void __launch_bounds__(256) biasRowsI8Kernel(GemmParams p) {
     const size_t idx = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (idx >= size_t(p.M) * p.N) return;
     const int m = int(idx / p.N), n = int(idx % p.N);
-    const int8_t *x = static_cast<const int8_t *>(p.x) + size_t(m) * p.K;
-    const int8_t *w = static_cast<const int8_t *>(p.w) + size_t(n) * p.K;
-    int sum = 0;
-    for (int k = 0; k < p.K; ++k) sum += int(x[k]) * int(w[k]);
-    float v = float(sum) * (p.xs[m] * p.ws[n]);
+    float v = 0.f * (p.xs[m] * p.ws[n]);
     if (p.bias) v += loadElem<O>(p.bias, n);
     storeElem<O>(p.y, idx, v);
 }
@@ -1248,8 +1264,13 @@ __global__ void __launch_bounds__(256) gemmRowsI8Kernel(GemmParams p) {
 // bytes, and a 64-k step of them takes an MFMA the time of a 32-k one), so the
 // 16-bit plans and lines are theirs at K / 2.
 bool tiledI8(const void *x, const void *w, int K) {
-    return K > 0 && K % 16 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) % 16 == 0;
+    return K % 16 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) % 16 == 0;
 }
+// Other operands are padded into the workspace first (behind the partials).
+int paddedK(int K) { return (K + 15) / 16 * 16; }
+
+// The partials' share of the workspace, in whole 16 B.
+size_t partialBytes(int M, int N, int K) { return (linearWorkspaceBytes(ElemType::BF16, M, N, K / 2) + 15) / 16 * 16; }
 
 template <ElemType O>
 void linearI8As(void *y, const int8_t *x, const float *xs, const int8_t *w, const float *ws, const void *bias, int M,
@@ -1262,14 +1283,25 @@ void linearI8As(void *y, const int8_t *x, const float *xs, const int8_t *w, cons
     p.N = N;
     p.K = K;
     p.ldy = N;
-    if (!tiledI8(x, w, K)) {
+    if (K == 0) {
         p.y = y;
-        p.x = x;
         p.xs = xs;
         p.M = M;
-        hipLaunchKernelGGL(gemmRowsI8Kernel<O>, dim3(unsigned((size_t(M) * N + 255) / 256)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(biasRowsI8Kernel<O>, dim3(unsigned((size_t(M) * N + 255) / 256)), dim3(256), 0, s, p);
         HIP_CHECK(hipGetLastError());
         return;
+    }
+    if (!tiledI8(x, w, K)) {
+        const int Kp = paddedK(K);
+        int8_t *to = static_cast<int8_t *>(workspace) + partialBytes(M, N, Kp);
+        const size_t pieces = (size_t(M) + N) * (Kp / 16);
+        hipLaunchKernelGGL(padRowsKernel, dim3(unsigned((pieces + 255) / 256)), dim3(256), 0, s, to, x, w, M, N, K, Kp);
+        HIP_CHECK(hipGetLastError());
+        x = to;
+        w = to + size_t(M) * Kp;
+        K = Kp;
+        p.w = w;
+        p.K = K;
     }
     const int rows_per_launch = rowsPerLaunch(ElemType::BF16, M, K / 2);
     for (int r0 = 0; r0 < M; r0 += rows_per_launch) {
@@ -1318,13 +1350,15 @@ void linearI8As(void *y, const int8_t *x, const float *xs, const int8_t *w, cons
 } // namespace
 
 size_t linearI8WorkspaceBytes(const int8_t *x, const int8_t *w, int M, int N, int K) {
-    return tiledI8(x, w, K) ? linearWorkspaceBytes(ElemType::BF16, M, N, K / 2) : 0;
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const int Kp = paddedK(K);
+    return partialBytes(M, N, Kp) + (tiledI8(x, w, K) ? 0 : (size_t(M) + N) * Kp);
 }
 
 void linearI8(void *y, const int8_t *x, const float *xs, const int8_t *w, const float *ws, const void *bias, ElemType t,
               int M, int N, int K, void *stream, void *workspace) {
     if (M <= 0 || N <= 0) return;
-    LLAISYS_CHECK(size_t(N) * K < kMaxBufferBytes || !tiledI8(x, w, K),
+    LLAISYS_CHECK(size_t(N) * paddedK(K) < kMaxBufferBytes,
                   "linear_i8: the weight (" << N << " x " << K << ") must be under 2 GiB");
     auto s = static_cast<hipStream_t>(stream);
     switch (t) {

@@ -177,7 +177,8 @@ void pagedCopyBlocksF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *
 void quantizeRows(int8_t *q, float *scale, const void *x, ElemType t, int M, int K, void *stream);
 // y[M, N] = (x . w^T) * (xs[m] * ws[n]) (+ bias[n]) for x [M, K], w [N, K]
 // (gemm.hip), the products summed in 32-bit integers (K <= kLinearI8MaxK), one
-// rounding to t. Split K leaves integer partials in `workspace`.
+// rounding to t. Split K leaves integer partials in `workspace`; operands whose
+// rows are not whole, aligned 16 B pieces are padded into it first.
 constexpr int kLinearI8MaxK = 131071; // 128 * 128 * K < 2^31
 size_t linearI8WorkspaceBytes(const int8_t *x, const int8_t *w, int M, int N, int K);
 void linearI8(void *y, const int8_t *x, const float *xs, const int8_t *w, const float *ws, const void *bias, ElemType t,

@@ -114,9 +114,43 @@ def test_products(device, dtype, M, N, K):
     (129, 520, 8960, torch.bfloat16, True), (300, 1537, 528, torch.float16, False), (777, 2048, 1536, torch.bfloat16, True),
     (1024, 1000, 4096, torch.float32, False), (2050, 4100, 656, torch.bfloat16, True), (8192, 1536, 1536, torch.bfloat16, False),
     (257, 300, 130, torch.bfloat16, True), (1030, 514, 16, torch.float32, True), (5, 1536, 16384, torch.bfloat16, False),
+    (2000, 4100, 129, torch.bfloat16, True), (9, 3000, 1001, torch.float16, False), (600, 700, 4099, torch.float32, True),
 ])
 def test_larger_products(M, N, K, dtype, bias):
     check_product("amd", M, N, K, dtype, bias)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("off", [1, 4, 16])
+@pytest.mark.parametrize("M, N, K", [(3, 40, 32), (130, 100, 96)])
+def test_operands_that_begin_anywhere(device, off, M, N, K):
+    """Views into larger buffers: contiguous, but not on a 16 B boundary."""
+    g = torch.Generator().manual_seed(off + M)
+    q, w = (torch.randint(-127, 128, (n, K), dtype=torch.int8, generator=g) for n in (M, N))
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16)
+    one = lambda n: give(torch.ones(n), device)  # noqa: E731
+
+    def view(t, dtype):
+        flat = torch.zeros(off + t.numel(), dtype=dtype)
+        flat[off:] = t.reshape(-1)
+        return give(flat, device).slice(0, off, off + t.numel()).view(*t.shape)
+
+    want = q.double() @ w.double().t()
+    for a, b in ((view(q, torch.int8), give(w, device)), (give(q, device), view(w, torch.int8))):
+        y = view(torch.zeros(M, N), torch.float32)
+        L.Ops.linear_i8(y, a, one(M), b, one(N))
+        flat = y.view(M * N)
+        out = give(torch.zeros(M * N), device)
+        L.Ops.rearrange(out, flat)
+        assert (take(out).double().view(M, N) == want).all()
+    codes, scale = view(torch.zeros(M, K), torch.int8), give(torch.zeros(M), device)
+    L.Ops.quantize_rows(codes, scale, view(x, torch.bfloat16))
+    out = give(torch.zeros(M, N), device)
+    L.Ops.linear_i8(out, codes, scale, give(w, device), one(N))
+    wq, ws = quantize64(x)
+    np.testing.assert_array_equal(take(scale).numpy(), ws)
+    dot = torch.from_numpy(wq).double() @ w.double().t() * torch.from_numpy(ws).double()[:, None]
+    assert ((take(out).double() - dot).abs() <= 4 * 2.0 ** -24 * dot.abs()).all()
 
 
 @pytest.mark.parametrize("device", DEVICES)
