@@ -83,8 +83,22 @@ void pagedDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_t
 // unit (55 GB/s): 1 x 768 10.2 / 9.6; with 128 units and more every CU has
 // one, and it lies further out: 64 x 300-800 11.3 / 13.4, 64 x 600-1024 13.2 /
 // 15.3.
-inline bool unitDecodeTakes(int B, int nkvh, int max_pages) {
-    return max_pages <= ((long long)B * nkvh >= 128 ? 64 : 44);
+// 8-bit pages, with f8UnitWaves waves a unit instead of two (us, this / stream-K):
+// 1 x 700 tokens 7.8 / 10.3, 1 x 1200 10.0 / 11.3, 1 x 1800 12.6 / 11.8, 16 x 1000
+// 10.0 / 12.3, 16 x 1300 12.1 / 12.6, 32 x 1500 13.0 / 14.9, 32 x 2000 16.0 / 15.7,
+// 64 x 600-1024 10.3 / 14.4, 64 x 100-2000 16.0 / 16.2, 64 x 2000 16.4 / 20.0, 128 x
+// 2000 23.4 / 29.4, 64 x 500-4000 27.1 / 21.8.
+inline bool unitDecodeTakes(int B, int nkvh, int max_pages, bool f8 = false) {
+    const long long units = (long long)B * nkvh;
+    if (f8) return max_pages <= (units >= 128 ? 128 : units >= 64 ? 96 : 80);
+    return max_pages <= (units >= 128 ? 64 : 44);
+}
+// Waves of a unit of 8-bit pages: their merge takes three steps instead of two,
+// which the shorter stream pays for where few units have many pages (us, 8 / 4:
+// 1 x 300 tokens 6.1 / 5.9, 1 x 1000 8.8 / 9.4, 1 x 1800 12.6 / 14.4, 16 x 1000 10.4 /
+// 10.0, 64 x 600-1024 11.1 / 10.3). With two, 1 x 700 takes 10.8 instead of 7.8.
+inline int f8UnitWaves(int B, int nkvh, int max_pages) {
+    return (long long)B * nkvh <= 16 && max_pages > 48 ? 8 : 4;
 }
 
 // pagedDecodeUnits with the decode step's QKV epilogue fused in (one token per

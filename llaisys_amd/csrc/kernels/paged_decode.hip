@@ -606,12 +606,13 @@ struct RopeArgs {
     bool keep_invalid;  // an invalid length leaves its output rows alone (else zeros)
 };
 
-template <bool OUT_F32, int NSTAGE, bool ROPE, class KV = KvBf16>
-__global__ void __launch_bounds__(64 * kUnitWaves)
+template <bool OUT_F32, int NSTAGE, bool ROPE, class KV = KvBf16, int UW = kUnitWaves>
+__global__ void __launch_bounds__(64 * UW)
     __attribute__((amdgpu_waves_per_eu(NSTAGE == 2 ? 2 : 1, NSTAGE == 2 ? 2 : 1)))
         decodeUnitKernel(DecodeArgs a, RopeArgs r) {
-    __shared__ f32x4 part_o[kUnitWaves - 1][8][64];
-    __shared__ float part_ml[kUnitWaves - 1][2][64];
+    static_assert((UW & (UW - 1)) == 0, "the merge halves the waves");
+    __shared__ f32x4 part_o[UW / 2][8][64];
+    __shared__ float part_ml[UW / 2][2][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int n = lane & 15;
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
         xr.load(r.x ? r.x + size_t(b) * r.hs : prow, xd);
     };
     // The waves take the unit's page pairs in turn: wave w owns pairs
-    // w, w + kUnitWaves, ... (its k-th pair is unit pair w + kUnitWaves k).
+    // w, w + UW, ... (its k-th pair is unit pair w + UW k).
     // So a wave's first block-table window does not depend on the length,
     // and its loads go out beside the length's: the first pages wait for
     // one memory round trip before them instead of two.
@@ -658,7 +659,7 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     // selects page A for a missing page B, and clamps to the wave's count).
     int base = 0, cnt = 0, bidA = 0, bidB = 0;
     auto loadWindow = [&]() {
-        const int pa = 2 * (wave + kUnitWaves * (base + lane));
+        const int pa = 2 * (wave + UW * (base + lane));
         bidA = row[min(pa, a.max_pages - 1)];
         bidB = row[min(pa + 1, a.max_pages - 1)];
     };
@@ -671,7 +672,7 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     c = __builtin_amdgcn_readfirstlane(c);
     const int np = (c + 15) >> 4;
     const int npr = (np + 1) >> 1;
-    const int nw = npr > wave ? (npr - wave + kUnitWaves - 1) / kUnitWaves : 0; // this wave's pairs
+    const int nw = npr > wave ? (npr - wave + UW - 1) / UW : 0; // this wave's pairs
     cnt = min(kPairsPerWave, nw);
     Acc acc;
     acc.reset();
@@ -686,7 +687,7 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     // pair again, an L2 hit, so loads are never conditional).
     auto issue = [&](int st, int k) {
         const int kk = max(min(k, cnt - 1), 0);
-        const int j = wave + kUnitWaves * (base + kk); // unit pair
+        const int j = wave + UW * (base + kk); // unit pair
         int bA = __builtin_amdgcn_readlane(bidA, kk);
         int bB = 2 * j + 1 < np ? __builtin_amdgcn_readlane(bidB, kk) : bA;
         const bool bad = unsigned(bA) >= unsigned(a.num_blocks) || unsigned(bB) >= unsigned(a.num_blocks);
@@ -704,12 +705,12 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     // count in the same in-order counter as loads, so a store issued before
     // the loop would hold up the waits on every page issued after it.
     __shared__ __align__(16) uint16_t kflat[ROPE ? kHeadDim : 8], vflat[ROPE ? kHeadDim : 8];
-    const bool last_wave = ROPE && nw > 0 && (npr - 1) % kUnitWaves == wave;
+    const bool last_wave = ROPE && nw > 0 && (npr - 1) % UW == wave;
     const int tok = (c - 1) & 15;
     bool issued = false; // the first window's first stages already in flight
     float rs = 1.f;      // the row's 1/rms (ROPE)
     int blk = 0;         // the new token's block id (ROPE)
-    __shared__ float2 trig[ROPE ? kUnitWaves : 1][64];
+    __shared__ float2 trig[ROPE ? UW : 1][64];
     if constexpr (ROPE) {
         // Loads return in issue order, so the block-table window and the new
         // token's block id go out first: the wait for them before the first
@@ -792,7 +793,7 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
             for (int st = 0; st < NSTAGE; ++st) {
                 const int k = k0 + st;
                 if (k < cnt_c) {
-                    const int j = wave + kUnitWaves * (base + k);
+                    const int j = wave + UW * (base + k);
                     PairScales ps{};
                     if constexpr (KV::kScaled) ps = scales.of(k);
                     KV::template consume<decodeParts<OUT_F32>()>(acc, ring[st], ps, qop, 32 * j, c - 1, c,
@@ -843,27 +844,31 @@ __global__ void __launch_bounds__(64 * kUnitWaves)
     if (bad_block && lane == 0) atomicOr(a.err, kErrBadBlock);
     float lt = acc.l + __shfl_xor(acc.l, 16);
     lt += __shfl_xor(lt, 32);
-    if (wave > 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) part_o[wave - 1][i][lane] = acc.o[i];
-        part_ml[wave - 1][0][lane] = acc.m;
-        part_ml[wave - 1][1][lane] = lt;
-    }
-    __syncthreads();
-    if (wave > 0 || n >= G || (c == 0 && r.keep_invalid)) return;
+    // The upper half of the waves hand their state to the lower half, until
+    // wave 0 has it all.
     float M = acc.m, L = lt;
 #pragma unroll
-    for (int v = 0; v < kUnitWaves - 1; ++v) {
-        const float mv = part_ml[v][0][lane];
-        if (mv == -INFINITY) continue;
-        const float Mn = fmaxf(M, mv);
-        const float sa = exp2Fast(M - Mn);
-        const float sb = exp2Fast(mv - Mn);
-        L = L * sa + part_ml[v][1][lane] * sb;
+    for (int half = UW / 2; half > 0; half /= 2) {
+        if (half < UW / 2) __syncthreads(); // the states before have been read
+        if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc.o[i] = acc.o[i] * sa + part_o[v][i][lane] * sb;
-        M = Mn;
+            for (int i = 0; i < 8; ++i) part_o[wave - half][i][lane] = acc.o[i];
+            part_ml[wave - half][0][lane] = M;
+            part_ml[wave - half][1][lane] = L;
+        }
+        __syncthreads();
+        const float mv = wave < half ? part_ml[wave][0][lane] : -INFINITY;
+        if (mv != -INFINITY) {
+            const float Mn = fmaxf(M, mv);
+            const float sa = exp2Fast(M - Mn);
+            const float sb = exp2Fast(mv - Mn);
+            L = L * sa + part_ml[wave][1][lane] * sb;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc.o[i] = acc.o[i] * sa + part_o[wave][i][lane] * sb;
+            M = Mn;
+        }
     }
+    if (wave > 0 || n >= G || (c == 0 && r.keep_invalid)) return;
     const float inv = L > 0.f ? 1.f / L : 0.f; // no keys (invalid length): zeros
     if (!OUT_F32 && r.o_packed) {
         // Dims 16 i + 4 grp .. + 3 of head h G + n: one 8 B piece of the
@@ -1086,10 +1091,17 @@ void launchDecodeUnits(void *out, bool out_f32, const uint16_t *q, const uint16_
     auto s = static_cast<hipStream_t>(stream);
     const dim3 grid(unsigned(B) * unsigned(nkvh)), block(64 * kUnitWaves);
     if (k_scale) {
-        if (out_f32)
-            hipLaunchKernelGGL((decodeUnitKernel<true, 2, false, KvF8>), grid, block, 0, s, a, r);
+        auto launch = [&](auto f32, auto waves) {
+            constexpr int UW = decltype(waves)::value;
+            hipLaunchKernelGGL((decodeUnitKernel<decltype(f32)::value, 2, false, KvF8, UW>), grid, dim3(64 * UW), 0, s,
+                               a, r);
+        };
+        const std::integral_constant<int, 8> eight;
+        const std::integral_constant<int, 4> four;
+        if (f8UnitWaves(B, nkvh, max_pages) == 8)
+            out_f32 ? launch(std::true_type(), eight) : launch(std::false_type(), eight);
         else
-            hipLaunchKernelGGL((decodeUnitKernel<false, 2, false, KvF8>), grid, block, 0, s, a, r);
+            out_f32 ? launch(std::true_type(), four) : launch(std::false_type(), four);
     } else if (rope) {
         if (out_f32)
             hipLaunchKernelGGL((decodeUnitKernel<true, 2, true>), grid, block, 0, s, a, r);

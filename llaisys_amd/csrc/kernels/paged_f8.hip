@@ -5,6 +5,8 @@
 
 #include "../device/hip_check.hpp"
 
+#include <type_traits>
+
 namespace llaisys::kernels {
 
 namespace {
@@ -36,115 +38,130 @@ __device__ __forceinline__ float scaled(uint32_t bits, float f) {
 
 constexpr int kRowPitch = kHeadDim + 8; // LDS row of 128 bf16, 16 B on
 
-// One workgroup per (row, kv head); the row that begins a run of consecutive
-// slots of a block does the run's work, the others end at once. Two waves hold
-// the K page, two the V page, 16 B of it per thread. The largest magnitude of
-// the run's rows and the block's scale give the new scale; if it grew, every
-// code of the page is re-encoded. Bound by latency: slots, then rows and page
-// together, then the stores.
+// A workgroup looks at ROWS rows of one kv head and writes the runs of
+// consecutive slots of a block that begin among them, one after the other. Two
+// waves hold the K page, two the V page, 16 B of it per thread. The largest
+// magnitude of the run's rows and the block's scale give the new scale; if it
+// grew, every code of the page is re-encoded. Bound by latency: slots, then
+// rows and page together, then the stores. One row per workgroup where every
+// row begins a run (64 rows 3.5 us); eight where most only continue one and
+// 2048 workgroups hold them all at once (8170 rows, 2 kv heads: 12.2 us with
+// one, whose idle workgroups take eight rounds).
+template <int ROWS>
 __global__ void __launch_bounds__(256)
     appendF8Kernel(uint8_t *__restrict__ k_pool, uint8_t *__restrict__ v_pool, float *__restrict__ k_scale,
                    float *__restrict__ v_scale, const uint16_t *__restrict__ k_new, const uint16_t *__restrict__ v_new,
                    const int64_t *__restrict__ slots, int T, int nkvh, int num_blocks, int *err) {
+    static_assert(kF8LookBack + ROWS - 1 + kPageTokens <= 64, "a lane per slot");
     __shared__ __align__(16) uint16_t rows[2][kPageTokens][kRowPitch];
     __shared__ int tops[4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = blockIdx.x, h = blockIdx.y;
-    // Lane l: the slot of row r + l - kF8LookBack.
-    int64_t slot = -1;
-    const int seen = r + lane - kF8LookBack;
-    if (seen >= 0 && seen < T) slot = slots[seen];
-    const int64_t mine = __shfl(slot, kF8LookBack), prev = __shfl(slot, kF8LookBack - 1);
-    if (mine < 0) return;
-    const int64_t block = mine >> 4;
-    const int off = int(mine & 15);
-    if (block >= num_blocks) {
-        if (tid == 0 && h == 0) atomicOr(err, kErrBadBlock);
-        return;
-    }
-    if (__ballot(lane < kF8LookBack && slot >= 0 && (slot >> 4) == block)) {
-        // Within a run that began earlier, or a second run of the block.
-        if (prev + 1 != mine && tid == 0 && h == 0) atomicOr(err, kErrTooLong);
-        return;
-    }
-    const unsigned long long run =
-        __ballot(lane >= kF8LookBack && lane < kF8LookBack + kPageTokens - off && slot == mine + (lane - kF8LookBack));
-    const int n = __ffsll(~(run >> kF8LookBack)) - 1; // rows of the run
-
+    const int r0 = int(blockIdx.x) * ROWS, h = blockIdx.y;
     const bool is_v = wave >= 2;
     const int i = tid & 127;
-    uint8_t *page = (is_v ? v_pool : k_pool) + (size_t(block) * nkvh + h) * kF8PageBytes;
-    float *scale = (is_v ? v_scale : k_scale) + size_t(block) * nkvh + h;
-    const u32x4 old_codes = reinterpret_cast<const u32x4 *>(page)[i];
-    const float old_scale = *scale;
-    // Rows to LDS, by slot: thread (slot t, eighth p) moves 16 dims.
-    const int t = i >> 3, p = i & 7;
-    int top = 0;
-    if (t >= off && t < off + n) {
-        const uint16_t *src = (is_v ? v_new : k_new) + (size_t(r + t - off) * nkvh + h) * kHeadDim + p * 16;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const u32x4 x = reinterpret_cast<const u32x4 *>(src)[j];
-            *reinterpret_cast<u32x4 *>(&rows[is_v][t][p * 16 + 8 * j]) = x;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int lo = int(x[w] & 0x7fffu), hi = int((x[w] >> 16) & 0x7fffu);
-                top = max(top, lo < 0x7f80 ? lo : 0);
-                top = max(top, hi < 0x7f80 ? hi : 0);
-            }
+    // Lane l: the slot of row r0 + l - kF8LookBack.
+    int64_t slot = -1;
+    const int seen = r0 + lane - kF8LookBack;
+    if (seen >= 0 && seen < T) slot = slots[seen];
+    const int64_t prev = __shfl_up(slot, 1);
+    const bool begins = lane >= kF8LookBack && lane < kF8LookBack + ROWS && slot >= 0 &&
+                        !(prev >= 0 && prev + 1 == slot && (slot & 15) != 0);
+    bool again = false;
+    for (unsigned long long todo = __ballot(begins); todo; todo &= todo - 1) {
+        const int l = __ffsll(todo) - 1, r = r0 + l - kF8LookBack;
+        const int64_t mine = __shfl(slot, l);
+        const int64_t block = mine >> 4;
+        const int off = int(mine & 15);
+        if (block >= num_blocks) {
+            if (tid == 0 && h == 0) atomicOr(err, kErrBadBlock);
+            continue;
         }
-    }
-    top = waveMaxInt(top);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    top = max(tops[wave & 2], tops[wave | 1]);
-    const int was = off == 0 ? kF8LeastExp : f8ExpOfScale(old_scale);
-    const int now = max(was, f8ExpOf(top));
-    const float f = f8Exp2(-now);
-    const bool recode = now != was && off != 0;
-    const float fr = f8Exp2(max(was - now, -126));
-    u32x4 codes = old_codes;
-    if (recode) {
+        if (__ballot(lane < l && lane >= l - kF8LookBack && slot >= 0 && (slot >> 4) == block)) {
+            if (tid == 0 && h == 0) atomicOr(err, kErrTooLong); // a second run of the block
+            continue;
+        }
+        const unsigned long long run = __ballot(lane >= l && lane < l + kPageTokens - off && slot == mine + (lane - l));
+        const int n = __ffsll(~(run >> l)) - 1; // rows of the run
+
+        uint8_t *page = (is_v ? v_pool : k_pool) + (size_t(block) * nkvh + h) * kF8PageBytes;
+        float *scale = (is_v ? v_scale : k_scale) + size_t(block) * nkvh + h;
+        const u32x4 old_codes = reinterpret_cast<const u32x4 *>(page)[i];
+        const float old_scale = *scale;
+        // Rows to LDS, by slot: thread (slot t, eighth p) moves 16 dims.
+        const int t = i >> 3, p = i & 7;
+        int top = 0;
+        u32x4 x[2] = {};
+        if (t >= off && t < off + n) {
+            const uint16_t *src = (is_v ? v_new : k_new) + (size_t(r + t - off) * nkvh + h) * kHeadDim + p * 16;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) codes[w] = recode4(codes[w], fr);
-    }
-    bool store = recode;
-    if (!is_v) {
-        // 16 B of one token: dims 64 half + 8 g + (0..7) and 32 further.
-        const int tok = i & 15, half = i >> 6, g = (i >> 4) & 3;
-        if (tok >= off && tok < off + n) {
-            store = true;
+            for (int j = 0; j < 2; ++j) x[j] = reinterpret_cast<const u32x4 *>(src)[j];
+        }
+        if (again) __syncthreads(); // the run before has been read
+        again = true;
+        if (t >= off && t < off + n) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(&rows[0][tok][64 * half + 32 * j + 8 * g]);
+                *reinterpret_cast<u32x4 *>(&rows[is_v][t][p * 16 + 8 * j]) = x[j];
 #pragma unroll
-                for (int w = 0; w < 2; ++w)
-                    codes[2 * j + w] = encode4(scaled(x[2 * w] & 0xffff, f), scaled(x[2 * w] >> 16, f),
-                                               scaled(x[2 * w + 1] & 0xffff, f), scaled(x[2 * w + 1] >> 16, f));
+                for (int w = 0; w < 4; ++w) {
+                    const int lo = int(x[j][w] & 0x7fffu), hi = int((x[j][w] >> 16) & 0x7fffu);
+                    top = max(top, lo < 0x7f80 ? lo : 0);
+                    top = max(top, hi < 0x7f80 ? hi : 0);
+                }
             }
         }
-    } else {
-        // Four tokens 4 g + (0..3) of dims 64 half + 16 w + n16.
-        const int half = i >> 6, g = (i >> 4) & 3, n16 = i & 15;
-        uint32_t keep = 0xffffffffu; // bytes of tokens that are not new
+        top = waveMaxInt(top);
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        top = max(tops[wave & 2], tops[wave | 1]);
+        const int was = off == 0 ? kF8LeastExp : f8ExpOfScale(old_scale);
+        const int now = max(was, f8ExpOf(top));
+        const float f = f8Exp2(-now);
+        const bool recode = now != was && off != 0;
+        const float fr = f8Exp2(max(was - now, -126));
+        u32x4 codes = old_codes;
+        if (recode) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (4 * g + e >= off && 4 * g + e < off + n) keep &= ~(0xffu << (8 * e));
-        if (keep != 0xffffffffu) {
-            store = true;
+            for (int w = 0; w < 4; ++w) codes[w] = recode4(codes[w], fr);
+        }
+        bool store = recode;
+        if (!is_v) {
+            // 16 B of one token: dims 64 half + 8 g + (0..7) and 32 further.
+            const int tok = i & 15, half = i >> 6, g = (i >> 4) & 3;
+            if (tok >= off && tok < off + n) {
+                store = true;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                float x[4];
+                for (int j = 0; j < 2; ++j) {
+                    const u32x4 y = *reinterpret_cast<const u32x4 *>(&rows[0][tok][64 * half + 32 * j + 8 * g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[e] = (keep >> (8 * e)) & 1 ? 0.f : scaled(rows[1][4 * g + e][64 * half + 16 * w + n16], f);
-                codes[w] = (codes[w] & keep) | (encode4(x[0], x[1], x[2], x[3]) & ~keep);
+                    for (int w = 0; w < 2; ++w)
+                        codes[2 * j + w] = encode4(scaled(y[2 * w] & 0xffff, f), scaled(y[2 * w] >> 16, f),
+                                                   scaled(y[2 * w + 1] & 0xffff, f), scaled(y[2 * w + 1] >> 16, f));
+                }
+            }
+        } else {
+            // Four tokens 4 g + (0..3) of dims 64 half + 16 w + n16.
+            const int half = i >> 6, g = (i >> 4) & 3, n16 = i & 15;
+            uint32_t keep = 0xffffffffu; // bytes of tokens that are not new
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * g + e >= off && 4 * g + e < off + n) keep &= ~(0xffu << (8 * e));
+            if (keep != 0xffffffffu) {
+                store = true;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    float y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        y[e] = (keep >> (8 * e)) & 1 ? 0.f : scaled(rows[1][4 * g + e][64 * half + 16 * w + n16], f);
+                    codes[w] = (codes[w] & keep) | (encode4(y[0], y[1], y[2], y[3]) & ~keep);
+                }
             }
         }
+        if (store) reinterpret_cast<u32x4 *>(page)[i] = codes;
+        if (i == 0) *scale = f8Exp2(now);
     }
-    if (store) reinterpret_cast<u32x4 *>(page)[i] = codes;
-    if (i == 0) *scale = f8Exp2(now);
 }
 
 // ---------------------------------------------------------------- gather
@@ -227,9 +244,16 @@ void pagedAppendF8(uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_sc
                    const uint16_t *v_new, const int64_t *slots, int T, int nkvh, int num_blocks, int *err,
                    void *stream) {
     if (T == 0) return;
-    hipLaunchKernelGGL(appendF8Kernel, dim3(unsigned(T), unsigned(nkvh)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), k_pool, v_pool, k_scale, v_scale, k_new, v_new, slots, T,
-                       nkvh, num_blocks, err);
+    auto launch = [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value;
+        hipLaunchKernelGGL(appendF8Kernel<ROWS>, dim3(unsigned((T + ROWS - 1) / ROWS), unsigned(nkvh)), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), k_pool, v_pool, k_scale, v_scale, k_new, v_new, slots, T,
+                           nkvh, num_blocks, err);
+    };
+    if ((long long)T * nkvh <= 1024)
+        launch(std::integral_constant<int, 1>());
+    else
+        launch(std::integral_constant<int, 8>());
     HIP_CHECK(hipGetLastError());
 }
 

@@ -10,6 +10,7 @@
 // the row (16 B each) in registers from the search for the largest magnitude
 // to the codes; what goes past kPieces of them is read again, from the caches.
 #include "launch.hpp"
+#include "mfma_common.hpp"
 
 #include "../device/hip_check.hpp"
 
@@ -21,7 +22,7 @@ namespace llaisys::kernels {
 
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+using mfma::u32x4;
 
 template <ElemType T> struct Elem;
 template <> struct Elem<ElemType::BF16> { using type = __bf16; };
@@ -38,6 +39,19 @@ __device__ __forceinline__ int quantized(float x, float s, float inv) {
     if (twice > s || (twice == s && odd)) q += copysignf(1.f, rest);
     return int(fminf(fmaxf(q, -127.f), 127.f));
 }
+
+// The same where x inv is not next to a tie, which it says: the product plus
+// 1.5 * 2^23 has the nearest whole number in its low bits. inv is off by 2^-24
+// of itself, so |x| inv <= 127 by 2^-17 at most.
+constexpr float kShift = 12582912.f, kSure = 0.5f - 0x1p-16f;
+__device__ __forceinline__ uint32_t quantizedFast(float x, float inv, float &far) {
+    const float y = fmaf(x, inv, kShift);
+    far = fmaxf(far, fabsf(fmaf(x, inv, kShift - y)));
+    return __float_as_uint(y);
+}
+
+// Largest over the 64 lanes of numbers >= 0 (as bits, which order as they do).
+__device__ __forceinline__ uint32_t waveMax(uint32_t bits) { return uint32_t(mfma::waveMaxInt(int(bits))); }
 
 // A row by WAVES waves (WAVES == 1: four rows a workgroup). VEC: rows of whole
 // 16 B pieces, aligned; else piece by piece of one element.
@@ -80,8 +94,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
         for (int i = 0; i < kPieces; ++i) search(held[i]);
     }
     for (int p = tid + kPieces * THREADS; p < pieces; p += THREADS) search(load(p));
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), off)));
+    top = waveMax(top);
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = __uint_as_float(top);
         __syncthreads();
@@ -95,12 +108,32 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
     // Rows of very small values: the same quotients from larger numbers, whose inverse is finite.
     const float grow = most < 0x1p-60f ? 0x1p80f : 1.f, sg = s * grow, inv = 1.f / sg;
     const bool some = finite && s > 0.f;
+    // (A scale of few bits, next to underflow, gives quotients past 127.)
+    const bool plain = some && s >= 0x1p-110f;
     auto store = [&](int p, const Piece &r) {
         uint32_t w[EL > 4 ? 2 : 1] = {};
+        float far = plain ? 0.f : 1.f;
+        if (plain) {
+            uint32_t c[EL];
 #pragma unroll
-        for (int e = 0; e < EL; ++e) {
-            const int c = some ? quantized(float(r.e[e]) * grow, sg, inv) : 0;
-            w[e / 4] |= (uint32_t(c) & 0xffu) << (8 * (e & 3));
+            for (int e = 0; e < EL; ++e) c[e] = quantizedFast(float(r.e[e]) * grow, inv, far);
+#pragma unroll
+            for (int e = 0; e < EL; e += 4) {
+                if constexpr (EL >= 4)
+                    w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[e + 3], c[e + 2], 0x0c0c0400u),
+                                                     __builtin_amdgcn_perm(c[e + 1], c[e], 0x0c0c0400u), 0x05040100u);
+                else
+                    w[0] = c[e];
+            }
+        }
+        if (far > kSure) {
+#pragma unroll
+            for (int e = 0; e < (EL > 4 ? 2 : 1); ++e) w[e] = 0;
+#pragma unroll
+            for (int e = 0; e < EL; ++e) {
+                const int c = some ? quantized(float(r.e[e]) * grow, sg, inv) : 0;
+                w[e / 4] |= (uint32_t(c) & 0xffu) << (8 * (e & 3));
+            }
         }
         if constexpr (EL == 8)
             reinterpret_cast<uint2 *>(to)[p] = make_uint2(w[0], w[1]);

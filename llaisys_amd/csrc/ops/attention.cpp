@@ -337,7 +337,7 @@ void attendOnDevice(const char *op, const tensor_t &out, const tensor_t &q, cons
     const int nb = int(k_pool->shape()[0]);
     const float *ks = k_scale ? reinterpret_cast<const float *>(k_scale->data()) : nullptr;
     const float *vs = v_scale ? reinterpret_cast<const float *>(v_scale->data()) : nullptr;
-    if (!cu_q && !stream_k && K::unitDecodeTakes(int(B), int(nkvh), max_pages)) {
+    if (!cu_q && !stream_k && K::unitDecodeTakes(int(B), int(nkvh), max_pages, ks != nullptr)) {
         K::pagedDecodeUnits(out->data(), f32, qp, kp, vp, tab, ctx, int(B), int(nh), int(nkvh), max_pages, nb, scale,
                             rt.errorWord(), rt.stream(), nullptr, true, ks, vs);
         return;

@@ -94,6 +94,9 @@ def test_decode(device, dtype, nh, nkvh, lens):
 @pytest.mark.parametrize("lens, extra", [
     ([2000], 0), ([700], 60), ([9000, 3], 0), (list(range(600, 1024, 7)), 0), (list(range(1, 8192, 177)), 10),
     ([1] * 200, 3), (list(range(1, 300)), 100),
+    # on both sides of the lines between the kernels: tables of 48 and 49, 80 and 81, 96 and 97, 128 and 129 pages
+    ([768, 5], 0), ([769, 5], 0), ([1280] + [1] * 9, 0), ([1281] + [1] * 9, 0), ([1536] + [70] * 31, 0),
+    ([1537] + [70] * 31, 0), ([2048] + [33] * 63, 0), ([2049] + [33] * 63, 0),
 ])
 def test_decode_long_and_many(dtype, lens, extra):
     cache, table, q = case(4, lens, 12, 2, [1] * len(lens), extra_pages=extra, stale_nan=True)

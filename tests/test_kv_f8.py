@@ -44,6 +44,27 @@ def test_appended_runs(device, nkvh, ctx, new):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("nkvh", [1, 2])
+@pytest.mark.parametrize("seed", range(4))
+def test_large_batches_of_ragged_runs(device, nkvh, seed):
+    """Single tokens, short runs and chunks in one batch, rows without a slot between them."""
+    r = np.random.RandomState(seed)
+    ctx = r.randint(0, 100, 300)
+    new = np.where(r.rand(300) < 0.7, 1, r.randint(1, 40, 300))
+    table, blocks = table_of(seed, ctx + new)
+    cache = Cache(blocks, nkvh, seed)
+    pools = cache.device(device)
+    slots = slots_of(table, ctx, new)
+    gap = np.repeat(r.rand(300) < 0.05, new)  # sequences whose rows are not written
+    slots[gap] = -1
+    k, v = rows_of(seed, len(slots), nkvh)
+    append(device, pools, k, v, slots)
+    assert L.device_error_flags() == 0
+    cache.append(f64(k), f64(v), slots)
+    cache.check(*pools)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_scale_that_grows_token_by_token(device):
     """Sixteen appends to a block, each larger than the last by a factor that
     varies: the codes are those of the growing scale, and no value that stays
