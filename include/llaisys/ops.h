@@ -203,7 +203,8 @@ __C {
     __export void llaisysPagedKVCopyBlocksF8(llaisysTensor_t k_pool, llaisysTensor_t v_pool, llaisysTensor_t k_scale,
                                              llaisysTensor_t v_scale, llaisysTensor_t pairs);
     /* llaisysPagedAttention and llaisysPagedAttentionVarlen over the 8-bit pool:
-     * the same arguments otherwise, the softmax and the sums in 32 bits. */
+     * the same arguments otherwise, with a positive scale; the softmax and the
+     * sums in 32 bits. */
     __export void llaisysPagedAttentionF8(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool,
                                           llaisysTensor_t v_pool, llaisysTensor_t k_scale, llaisysTensor_t v_scale,
                                           llaisysTensor_t block_table, llaisysTensor_t ctx_len, float scale);

@@ -142,7 +142,7 @@ struct PagedAttentionPlan {
     int pages_per_split_min; // the persistent kernel may cut splits down to this
     size_t partial_bytes; // workspace for split records
 };
-PagedAttentionPlan planPrefill(int B, int T, int nkvh, int group, int max_pages);
+PagedAttentionPlan planPrefill(int B, int T, int nkvh, int group, int max_pages, bool f8 = false);
 // Whether pagedPrefill runs its persistent kernel (the work-queue counters
 // given, the batch's tables fit its LDS) and, then, whether that kernel also
 // takes the batch's single-query sequences (T != B), in which case the

@@ -45,10 +45,15 @@ namespace {
 using namespace mfma;
 
 constexpr int kXcds = 8;
-constexpr int kTiles = 2;                                    // query tiles per wave
-constexpr int kWaves = 8;                                    // waves (groups) per workgroup
-constexpr int kStagePairs = 2;                               // page pairs per LDS stage (one barrier each)
-constexpr int kRecordFloats = kTiles * 16 * (kHeadDim + 2); // O for the group's columns, then (m, l)
+constexpr int kStagePairs = 2; // page pairs per LDS stage (one barrier each)
+// A workgroup's waves (groups) and their query tiles; a record is O for a
+// group's columns, then (m, l).
+template <int WAVES, int TILES> struct Geo {
+    static constexpr int kWaves = WAVES, kTiles = TILES, kColumns = WAVES * TILES * 16;
+    static constexpr int kRecordFloats = TILES * 16 * (kHeadDim + 2);
+};
+using GeoBf16 = Geo<8, 2>;
+using GeoF8 = Geo<8, 2>;
 
 // bf16 parts of the prompt tiles' weights.
 template <bool OUT_F32> constexpr int weightParts() { return OUT_F32 ? 2 : 1; }
@@ -74,22 +79,23 @@ struct Args {
     float scale_log2;
 };
 
-__device__ __forceinline__ int groupsOf(const Args &a, int bb) {
+template <class GEO> __device__ __forceinline__ int groupsOf(const Args &a, int bb) {
     const int lq = a.cu_q[bb + 1] - a.cu_q[bb];
-    return lq >= 2 ? (((lq * a.G + 15) >> 4) + kTiles - 1) / kTiles : 0;
+    return lq >= 2 ? (((lq * a.G + 15) >> 4) + GEO::kTiles - 1) / GEO::kTiles : 0;
 }
 
 // Item `index` of the list where each sequence with Lq >= 2 contributes its
 // groups (blocks == false) or its blocks of kWaves groups (blocks == true):
 // its sequence b, index within the sequence, and the number of groups of the
 // sequences before b. Returns false past the last item. One wave.
+template <class GEO>
 __device__ bool locate(const Args &a, int index, bool blocks, int &b, int &local, int &group_base) {
     const int lane = threadIdx.x & 63;
     int remaining = index, groups_before = 0;
     for (int base = 0; base < a.B; base += 64) {
         const int bb = base + lane;
-        const int ng = bb < a.B ? groupsOf(a, bb) : 0;
-        const int ni = blocks ? (ng + kWaves - 1) / kWaves : ng;
+        const int ng = bb < a.B ? groupsOf<GEO>(a, bb) : 0;
+        const int ni = blocks ? (ng + GEO::kWaves - 1) / GEO::kWaves : ng;
         const int incl = waveInclusiveSum(ni), gincl = waveInclusiveSum(ng);
         const int total = __builtin_amdgcn_readlane(incl, 63);
         if (remaining < total) {
@@ -120,6 +126,7 @@ struct TileGeom {
     int b, group, q0, Lq, ctx, npages, nsplit;
 };
 
+template <class GEO>
 __device__ bool blockGeom(const Args &a, int b, int block, int pps, TileGeom &t, bool report) {
     t.b = b;
     t.q0 = a.cu_q[b];
@@ -129,7 +136,7 @@ __device__ bool blockGeom(const Args &a, int b, int block, int pps, TileGeom &t,
         if (report && (threadIdx.x & 63) == 0) atomicOr(a.err, kErrTooLong);
         return false;
     }
-    const int qi_max = min(t.Lq - 1, ((block + 1) * kWaves * kTiles * 16 - 1) / a.G);
+    const int qi_max = min(t.Lq - 1, ((block + 1) * GEO::kColumns - 1) / a.G);
     const int kv_len = t.ctx - t.Lq + qi_max + 1; // keys some column of the block sees
     t.npages = (kv_len + 15) >> 4;
     t.nsplit = (t.npages + pps - 1) / pps;
@@ -168,7 +175,7 @@ typedef u32x4 StageBuf[2][kStagePairs * 16 * 64]; // page pairs: K a, K b, V a, 
 // (groups block * kWaves .. + kWaves - 1 of its groups_b; group_base groups
 // before the sequence), pages [split * pps, ...) of its t.npages. Called by
 // every wave of the workgroup with the same arguments (it has barriers).
-template <bool OUT_F32, bool CHOOSE, class KV>
+template <bool OUT_F32, bool CHOOSE, class GEO>
 __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b, int block, int group_base, int h,
                                             int split, int pps, int groups_b, const TileGeom &t) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); // uniform: scalar branches on it
@@ -179,15 +186,15 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     const int p0 = split * pps;
     if (p0 >= t.npages) return;
     const int p1 = min(t.npages, p0 + pps);
-    const int group = block * kWaves + wave;        // this wave's group in the sequence
+    const int group = block * GEO::kWaves + wave;        // this wave's group in the sequence
     const bool active = group < groups_b;
 
     // Columns of the wave's tiles.
-    int qi[kTiles], g[kTiles], pos[kTiles];
-    bool col_ok[kTiles];
+    int qi[GEO::kTiles], g[GEO::kTiles], pos[GEO::kTiles];
+    bool col_ok[GEO::kTiles];
 #pragma unroll
-    for (int k = 0; k < kTiles; ++k) {
-        const int pair = (group * kTiles + k) * 16 + n;
+    for (int k = 0; k < GEO::kTiles; ++k) {
+        const int pair = (group * GEO::kTiles + k) * 16 + n;
         qi[k] = pair / G;
         g[k] = pair - qi[k] * G;
         col_ok[k] = active && qi[k] < t.Lq;
@@ -197,7 +204,7 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     // Smallest causal limit among the wave's real columns (wave-uniform).
     int min_pos = 0x7fffffff;
 #pragma unroll
-    for (int k = 0; k < kTiles; ++k) min_pos = min(min_pos, col_ok[k] ? pos[k] : 0x7fffffff);
+    for (int k = 0; k < GEO::kTiles; ++k) min_pos = min(min_pos, col_ok[k] ? pos[k] : 0x7fffffff);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) min_pos = min(min_pos, __shfl_xor(min_pos, off));
     min_pos = __builtin_amdgcn_readfirstlane(min_pos);
@@ -211,23 +218,10 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
         const int i = page - p0;
         return i < 64 ? __builtin_amdgcn_readlane(bid[0], i) : __builtin_amdgcn_readlane(bid[1], i - 64);
     };
-    // 8-bit pages: their scales the same way, of the pool that this wave stages.
-    float scales[2] = {0.f, 0.f};
-    if constexpr (KV::kScaled) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-            if (unsigned(bid[w]) < unsigned(a.num_blocks))
-                scales[w] = ((wave >> 1) & 2 ? a.v_scale : a.k_scale)[size_t(bid[w]) * a.nkvh + h];
-    }
-    auto scaleOf = [&](int page) {
-        const int i = page - p0;
-        return __uint_as_float(uint32_t(i < 64 ? __builtin_amdgcn_readlane(int(__float_as_uint(scales[0])), i)
-                                               : __builtin_amdgcn_readlane(int(__float_as_uint(scales[1])), i - 64)));
-    };
 
-    u32x4 qop[kTiles][4];
+    u32x4 qop[GEO::kTiles][4];
 #pragma unroll
-    for (int k = 0; k < kTiles; ++k) {
+    for (int k = 0; k < GEO::kTiles; ++k) {
         const uint16_t *qrow =
             a.q + (size_t(t.q0 + (col_ok[k] ? qi[k] : 0)) * a.nh + h * G + (col_ok[k] ? g[k] : 0)) * kHeadDim + grp * 8;
 #pragma unroll
@@ -244,12 +238,9 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     // V a, V b) and quarter (q % 4). Wave w stages slots w, w + kWaves, ...
     // Clamped: past the end it re-reads the last pair, so loads are never
     // conditional.
-    static_assert(16 % kWaves == 0, "the 16 quarters of a pair split evenly over the waves");
-    // (8-bit pages: 8 one-KiB halves, one per wave: part wave / 2, half wave % 2.)
-    static_assert(!KV::kScaled || kWaves == 8, "one half of an 8-bit page pair per wave");
-    constexpr int kPer = KV::kScaled ? 1 : 16 / kWaves;
+    static_assert(16 % GEO::kWaves == 0, "the 16 quarters of a pair split evenly over the waves");
+    constexpr int kPer = 16 / GEO::kWaves;
     u32x4 st[kStagePairs][kPer];
-    float st_scale[kStagePairs];
     auto stageLoad = [&](int pp) { // the kStagePairs pairs from page pp
 #pragma unroll
         for (int sp = 0; sp < kStagePairs; ++sp) {
@@ -260,15 +251,10 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
             bad_block |= bad;
             ba = bad ? 0 : ba;
             bb = bad ? 0 : bb;
-            const size_t oa = (size_t(ba) * a.nkvh + h) * KV::kPageVecs, ob = (size_t(bb) * a.nkvh + h) * KV::kPageVecs;
-            if constexpr (KV::kScaled) {
-                const int part = wave >> 1, half = wave & 1;
-                st[sp][0] = __builtin_nontemporal_load(((part & 2) ? vp : kp) + ((part & 1) ? ob : oa) + half * 64);
-                st_scale[sp] = scaleOf((part & 1) && q0 + 1 < p1 ? q0 + 1 : q0);
-            } else
+            const size_t oa = (size_t(ba) * a.nkvh + h) * 256, ob = (size_t(bb) * a.nkvh + h) * 256;
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
-                const int q = wave + kWaves * j, part = q >> 2, quarter = q & 3;
+                const int q = wave + GEO::kWaves * j, part = q >> 2, quarter = q & 3;
                 const u32x4 *base = (part & 2) ? vp : kp;
                 st[sp][j] = __builtin_nontemporal_load(base + ((part & 1) ? ob : oa) + quarter * 64);
             }
@@ -278,37 +264,26 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     // slot (8 + 2 s + h) of a pair holds, per lane, half h (dwords 2h, 2h+1)
     // of V page A's quarter s in its low 8 bytes and of page B's in its high 8.
     auto stageStore = [&](int buf) {
-        auto put = [&](u32x4 *pair, int part, int quarter, u32x4 v) {
-            if (part < 2) {
-                pair[(4 * part + quarter) * 64 + lane] = v;
-            } else {
-                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                u32x2 *half = reinterpret_cast<u32x2 *>(pair + (8 + 2 * quarter) * 64 + lane) + (part & 1);
-                half[0] = u32x2{v[0], v[1]};
-                half[64 * 2] = u32x2{v[2], v[3]}; // next slot, same lane
-            }
-        };
 #pragma unroll
-        for (int sp = 0; sp < kStagePairs; ++sp) {
-            u32x4 *pair = kvs[buf] + sp * 16 * 64;
-            if constexpr (KV::kScaled) { // widened on the way, so the rest of the loop is the bf16 pages'
-                u32x4 q0, q1;
-                widenHalf(q0, q1, st[sp][0], st_scale[sp]);
-                put(pair, wave >> 1, 2 * (wave & 1), q0);
-                put(pair, wave >> 1, 2 * (wave & 1) + 1, q1);
-            } else {
+        for (int sp = 0; sp < kStagePairs; ++sp)
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    const int q = wave + kWaves * j;
-                    put(pair, q >> 2, q & 3, st[sp][j]);
+            for (int j = 0; j < kPer; ++j) {
+                const int q = wave + GEO::kWaves * j, part = q >> 2, quarter = q & 3;
+                u32x4 *pair = kvs[buf] + sp * 16 * 64;
+                if (part < 2) {
+                    pair[q * 64 + lane] = st[sp][j];
+                } else {
+                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                    u32x2 *half = reinterpret_cast<u32x2 *>(pair + (8 + 2 * quarter) * 64 + lane) + (part & 1);
+                    half[0] = u32x2{st[sp][j][0], st[sp][j][1]};
+                    half[64 * 2] = u32x2{st[sp][j][2], st[sp][j][3]}; // next slot, same lane
                 }
             }
-        }
     };
 
-    Acc acc[kTiles];
+    Acc acc[GEO::kTiles];
 #pragma unroll
-    for (int k = 0; k < kTiles; ++k) acc[k].reset();
+    for (int k = 0; k < GEO::kTiles; ++k) acc[k].reset();
     constexpr int kStagePages = 2 * kStagePairs;
     stageLoad(p0);
     stageStore(0);
@@ -330,7 +305,7 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
 #pragma unroll
             for (int sg = 0; sg < kStagePairs; sg += kSoft) {
                 if (ps + 2 * sg >= p1) break;
-                float sv[kTiles][kSoft][8];
+                float sv[GEO::kTiles][kSoft][8];
 #pragma unroll
                 for (int j = 0; j < kSoft; ++j) {
                     const int pp = ps + 2 * (sg + j);
@@ -345,19 +320,19 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
                         ka[s] = src[(0 * 4 + s) * 64 + lane];
                         kb[s] = src[(1 * 4 + s) * 64 + lane];
                     }
-                    int lim[kTiles];
+                    int lim[GEO::kTiles];
 #pragma unroll
-                    for (int k = 0; k < kTiles; ++k) lim[k] = hasA ? pos[k] : -1;
-                    float svj[kTiles][8];
-                    pairScoresN<kTiles>(svj, ka, kb, qop, pp * 16, lim, hasB, grp, full);
+                    for (int k = 0; k < GEO::kTiles; ++k) lim[k] = hasA ? pos[k] : -1;
+                    float svj[GEO::kTiles][8];
+                    pairScoresN<GEO::kTiles>(svj, ka, kb, qop, pp * 16, lim, hasB, grp, full);
 #pragma unroll
-                    for (int k = 0; k < kTiles; ++k)
+                    for (int k = 0; k < GEO::kTiles; ++k)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) sv[k][j][e] = svj[k][e];
                 }
-                PairP<weightParts<OUT_F32>()> P[kTiles][kSoft];
+                PairP<weightParts<OUT_F32>()> P[GEO::kTiles][kSoft];
 #pragma unroll
-                for (int k = 0; k < kTiles; ++k) softmaxUpdate<weightParts<OUT_F32>(), kSoft>(acc[k], sv[k], P[k], a.scale_log2);
+                for (int k = 0; k < GEO::kTiles; ++k) softmaxUpdate<weightParts<OUT_F32>(), kSoft>(acc[k], sv[k], P[k], a.scale_log2);
 #pragma unroll
                 for (int j = 0; j < kSoft; ++j) {
                     const int pp = ps + 2 * (sg + j);
@@ -372,7 +347,7 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
                     }
                     maskStaleVPacked(v0, v1, pp * 16, t.ctx, hasB, grp);
 #pragma unroll
-                    for (int k = 0; k < kTiles; ++k) accumulatePVPacked<weightParts<OUT_F32>()>(acc[k], v0, v1, P[k][j]);
+                    for (int k = 0; k < GEO::kTiles; ++k) accumulatePVPacked<weightParts<OUT_F32>()>(acc[k], v0, v1, P[k][j]);
                 }
             }
         }
@@ -381,9 +356,9 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
     if (bad_block && lane == 0) atomicOr(a.err, kErrBadBlock);
     if (!active) return;
     const int unit = (group_base + group) * a.nkvh + h;
-    float *rec = a.records + (size_t(unit) * splitStride<CHOOSE>(a, pps) + split) * kRecordFloats;
+    float *rec = a.records + (size_t(unit) * splitStride<CHOOSE>(a, pps) + split) * GEO::kRecordFloats;
 #pragma unroll
-    for (int k = 0; k < kTiles; ++k) {
+    for (int k = 0; k < GEO::kTiles; ++k) {
         float lt = acc[k].l + __shfl_xor(acc[k].l, 16);
         lt += __shfl_xor(lt, 32);
         if (!col_ok[k]) continue;
@@ -397,19 +372,283 @@ __device__ __forceinline__ void prefillItem(const Args &a, StageBuf &kvs, int b,
         const int c = k * 16 + n; // column within the group
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int at = (i * kTiles * 16 + c) * 16 + grp * 4;
+            const int at = (i * GEO::kTiles * 16 + c) * 16 + grp * 4;
             if (CHOOSE && pps < a.pps)
                 storeRecordO<true>(rec, at, acc[k].o[i]);
             else
                 storeRecordO<OUT_F32>(rec, at, acc[k].o[i]);
         }
         if (grp == 0)
-            *reinterpret_cast<float2 *>(rec + kTiles * 16 * kHeadDim + 2 * c) = make_float2(acc[k].m, lt);
+            *reinterpret_cast<float2 *>(rec + GEO::kTiles * 16 * kHeadDim + 2 * c) = make_float2(acc[k].m, lt);
     }
 }
 
-template <bool OUT_F32, class KV>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) prefillKernel(Args a) {
+// The same of 8-bit pages, which are widened once, on their way to LDS, where
+// they are as the bf16 pages are. The sums of the weights come from the matrix
+// cores too (a row of ones beside V), of the weights as rounded, so their
+// rounding moves the quotient's two sides alike; and lanes compare their scores
+// only when a column's maximum has to move.
+template <bool OUT_F32, bool CHOOSE, class GEO>
+__device__ __forceinline__ void prefillItemF8(const Args &a, StageBuf &kvs, int b, int block, int group_base, int h,
+                                              int split, int pps, int groups_b, const TileGeom &t) {
+    constexpr int TILES = GEO::kTiles, PARTS = weightParts<OUT_F32>();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int n = lane & 15;
+    const int grp = lane >> 4;
+    const int G = a.G;
+    const int p0 = split * pps;
+    if (p0 >= t.npages) return;
+    const int p1 = min(t.npages, p0 + pps);
+    const int group = block * GEO::kWaves + wave; // this wave's group in the sequence
+    const bool active = group < groups_b;
+
+    int qi[TILES], g[TILES], pos[TILES];
+    bool col_ok[TILES];
+    int min_pos = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < TILES; ++k) {
+        const int pair = (group * TILES + k) * 16 + n;
+        qi[k] = pair / G;
+        g[k] = pair - qi[k] * G;
+        col_ok[k] = active && qi[k] < t.Lq;
+        pos[k] = col_ok[k] ? t.ctx - t.Lq + qi[k] : -1;
+        min_pos = min(min_pos, col_ok[k] ? pos[k] : 0x7fffffff);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) min_pos = min(min_pos, __shfl_xor(min_pos, off));
+    min_pos = __builtin_amdgcn_readfirstlane(min_pos);
+
+    // Block ids of the split's pages, page p0 + i in lane i % 64 of bid[i / 64],
+    // and the scales of the part of the pairs that this wave stages.
+    constexpr int HALVES = 8 / GEO::kWaves; // one-KiB halves of a pair per wave
+    const int part = wave * HALVES / 2, half0 = wave * HALVES % 2; // part: K of page A, of B, V of A, of B
+    const bool odd = part & 1;
+    const u32x4 *pool = reinterpret_cast<const u32x4 *>(part & 2 ? a.v_pool : a.k_pool) + lane;
+    int bid[2] = {0, 0};
+    float scales[2] = {0.f, 0.f};
+    bool bad_block = false;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+        if (lane + 64 * w < p1 - p0) {
+            bid[w] = a.table[size_t(t.b) * a.max_pages + p0 + 64 * w + lane];
+            if (unsigned(bid[w]) >= unsigned(a.num_blocks)) {
+                bad_block = true;
+                bid[w] = 0;
+            }
+            scales[w] = (part & 2 ? a.v_scale : a.k_scale)[size_t(bid[w]) * a.nkvh + h];
+        }
+
+    u32x4 qop[TILES][4];
+#pragma unroll
+    for (int k = 0; k < TILES; ++k) {
+        const uint16_t *qrow =
+            a.q + (size_t(t.q0 + (col_ok[k] ? qi[k] : 0)) * a.nh + h * G + (col_ok[k] ? g[k] : 0)) * kHeadDim + grp * 8;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) qop[k][s] = *reinterpret_cast<const u32x4 *>(qrow + 32 * s);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) qop[k][s] = col_ok[k] ? qop[k][s] : u32x4{0, 0, 0, 0};
+    }
+
+    const int last_pair = p0 + ((p1 - 1 - p0) & ~1);
+    u32x4 st[kStagePairs][HALVES];
+    float st_scale[kStagePairs];
+    // Past the end it re-reads the last pair, so loads are never conditional.
+    auto stageLoad = [&](int pp) {
+#pragma unroll
+        for (int sp = 0; sp < kStagePairs; ++sp) {
+            const int q0 = min(pp + 2 * sp, last_pair);
+            const int i = (odd && q0 + 1 < p1 ? q0 + 1 : q0) - p0;
+            const int blk = i < 64 ? __builtin_amdgcn_readlane(bid[0], i) : __builtin_amdgcn_readlane(bid[1], i - 64);
+            const int sc = i < 64 ? __builtin_amdgcn_readlane(int(__float_as_uint(scales[0])), i)
+                                  : __builtin_amdgcn_readlane(int(__float_as_uint(scales[1])), i - 64);
+            st_scale[sp] = __uint_as_float(uint32_t(sc));
+            const size_t at = (size_t(blk) * a.nkvh + h) * KvF8::kPageVecs;
+#pragma unroll
+            for (int j = 0; j < HALVES; ++j) st[sp][j] = __builtin_nontemporal_load(pool + at + (half0 + j) * 64);
+        }
+    };
+    // The layout of prefillItem's stages.
+    auto stageStore = [&](int buf) {
+#pragma unroll
+        for (int sp = 0; sp < kStagePairs; ++sp) {
+            u32x4 *pair = kvs[buf] + sp * 16 * 64;
+#pragma unroll
+            for (int hj = 0; hj < HALVES; ++hj) {
+                u32x4 q[2];
+                widenHalf(q[0], q[1], st[sp][hj], st_scale[sp]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int quarter = 2 * (half0 + hj) + j;
+                    if (!(part & 2)) {
+                        pair[(4 * odd + quarter) * 64 + lane] = q[j];
+                    } else {
+                        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                        u32x2 *to = reinterpret_cast<u32x2 *>(pair + (8 + 2 * quarter) * 64 + lane) + odd;
+                        to[0] = u32x2{q[j][0], q[j][1]};
+                        to[64 * 2] = u32x2{q[j][2], q[j][3]}; // next slot, same lane
+                    }
+                }
+            }
+        }
+    };
+
+    f32x4 o[TILES][8], l[TILES];
+    float m[TILES];
+#pragma unroll
+    for (int k = 0; k < TILES; ++k) {
+        m[k] = -INFINITY;
+        l[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const bf16x8 ones = asBf16(u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+    constexpr int kStagePages = 2 * kStagePairs;
+    stageLoad(p0);
+    stageStore(0);
+    __syncthreads();
+    stageLoad(p0 + kStagePages);
+    for (int i = 0, ps = p0; ps < p1; ++i, ps += kStagePages) {
+        stageStore((i + 1) & 1);
+        stageLoad(ps + 2 * kStagePages);
+        if (active) {
+            // The stage's pairs as one step of the softmax: their scores, the
+            // maximum, the weights, then P.V pair by pair (fp32 outputs, whose
+            // weights are two parts: a pair a step).
+            constexpr int SOFT = OUT_F32 ? 1 : kStagePairs;
+#pragma unroll
+            for (int sg = 0; sg < kStagePairs; sg += SOFT) {
+                if (ps + 2 * sg >= p1) break;
+                float sv[SOFT][TILES][8];
+#pragma unroll
+                for (int j = 0; j < SOFT; ++j) {
+                    const int pp = ps + 2 * (sg + j);
+                    const u32x4 *src = kvs[i & 1] + (sg + j) * 16 * 64;
+                    const bool hasB = pp + 1 < p1;
+                    // Every key of the pair visible to every column of the wave: no per-key mask.
+                    const bool full = hasB && pp * 16 + 31 <= min_pos && pp * 16 + 32 <= t.ctx;
+                    u32x4 ka[4], kb[4];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        ka[s] = src[s * 64 + lane];
+                        kb[s] = src[(4 + s) * 64 + lane];
+                    }
+                    int lim[TILES];
+#pragma unroll
+                    for (int k = 0; k < TILES; ++k) lim[k] = pp < p1 ? pos[k] : -1;
+                    pairScoresN<TILES>(sv[j], ka, kb, qop, pp * 16, lim, hasB, grp, full);
+                }
+                u32x4 v0[4], v1[4];
+                auto readV = [&](int j) {
+                    const u32x4 *src = kvs[i & 1] + (sg + j) * 16 * 64;
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        v0[s] = src[(8 + 2 * s) * 64 + lane];
+                        v1[s] = src[(9 + 2 * s) * 64 + lane];
+                    }
+                };
+                readV(0);
+                // Lazy rescale (softmaxUpdate's): a lane's own scores tell whether
+                // its column's maximum has to move; only then do lanes compare.
+                float most[TILES];
+                bool moves = false;
+#pragma unroll
+                for (int k = 0; k < TILES; ++k) {
+                    most[k] = sv[0][k][0];
+#pragma unroll
+                    for (int j = 0; j < SOFT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) most[k] = fmaxf(most[k], sv[j][k][e]);
+                    moves = moves || most[k] * a.scale_log2 > m[k] + 8.f;
+                }
+                if (__builtin_amdgcn_ballot_w64(moves) != 0) {
+#pragma unroll
+                    for (int k = 0; k < TILES; ++k) {
+                        const float mt = fmaxf(m[k], maxOverGroups(most[k]) * a.scale_log2);
+                        const float alpha = exp2Fast(m[k] - (mt == -INFINITY ? 0.f : mt));
+                        l[k] *= alpha;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[k][e] *= alpha;
+                        m[k] = mt;
+                    }
+                }
+                PairP<PARTS> P[SOFT][TILES];
+#pragma unroll
+                for (int j = 0; j < SOFT; ++j)
+#pragma unroll
+                    for (int k = 0; k < TILES; ++k) {
+                        const float mu = m[k] == -INFINITY ? 0.f : m[k];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float rest = exp2Fast(__builtin_fmaf(sv[j][k][e], a.scale_log2, -mu));
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part) {
+                                const __bf16 x = (__bf16)rest;
+                                P[j][k].part[part][e] = x;
+                                rest -= (float)x;
+                            }
+                        }
+                    }
+#pragma unroll
+                for (int j = 0; j < SOFT; ++j) {
+                    const int pp = ps + 2 * (sg + j);
+                    if (pp >= p1) break;
+                    if (j > 0) readV(j);
+                    maskStaleVPacked(v0, v1, pp * 16, t.ctx, pp + 1 < p1, grp);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                        for (int k = 0; k < TILES; ++k) {
+#pragma unroll
+                            for (int s = 0; s < 4; ++s) {
+                                o[k][2 * s] = mfma::mfma(asBf16(v0[s]), P[j][k].part[part], o[k][2 * s]);
+                                o[k][2 * s + 1] = mfma::mfma(asBf16(v1[s]), P[j][k].part[part], o[k][2 * s + 1]);
+                            }
+                            l[k] = mfma::mfma(ones, P[j][k].part[part], l[k]);
+                        }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (__builtin_amdgcn_ballot_w64(bad_block) != 0 && lane == 0) atomicOr(a.err, kErrBadBlock);
+    if (!active) return;
+    const int unit = (group_base + group) * a.nkvh + h;
+    float *rec = a.records + (size_t(unit) * splitStride<CHOOSE>(a, pps) + split) * GEO::kRecordFloats;
+#pragma unroll
+    for (int k = 0; k < TILES; ++k) {
+        if (!col_ok[k]) continue;
+        if (t.nsplit == 1) {
+            const size_t row = (size_t(t.q0 + qi[k]) * a.nh + h * G + g[k]) * kHeadDim;
+            const float inv = 1.f / l[k][0];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) storeOut<OUT_F32>(a.out, row, e, grp, o[k][e] * inv);
+            continue;
+        }
+        const int c = k * 16 + n; // column within the group
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int at = (e * TILES * 16 + c) * 16 + grp * 4;
+            if (CHOOSE && pps < a.pps)
+                storeRecordO<true>(rec, at, o[k][e]);
+            else
+                storeRecordO<OUT_F32>(rec, at, o[k][e]);
+        }
+        if (grp == 0) *reinterpret_cast<float2 *>(rec + TILES * 16 * kHeadDim + 2 * c) = make_float2(m[k], l[k][0]);
+    }
+}
+
+template <bool OUT_F32, bool CHOOSE, class KV, class GEO>
+__device__ __forceinline__ void prefillOne(const Args &a, StageBuf &kvs, int b, int block, int group_base, int h,
+                                           int split, int pps, int groups_b, const TileGeom &t) {
+    if constexpr (KV::kScaled)
+        prefillItemF8<OUT_F32, CHOOSE, GEO>(a, kvs, b, block, group_base, h, split, pps, groups_b, t);
+    else
+        prefillItem<OUT_F32, CHOOSE, GEO>(a, kvs, b, block, group_base, h, split, pps, groups_b, t);
+}
+
+template <bool OUT_F32, class KV, class GEO>
+__global__ void __launch_bounds__(64 * GEO::kWaves) __attribute__((amdgpu_waves_per_eu(GEO::kWaves / 4, GEO::kWaves / 4))) prefillKernel(Args a) {
     __shared__ StageBuf kvs;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int split = blockIdx.x / a.block_units_padded;
@@ -417,18 +656,18 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     if (wunit >= a.block_units) return;
     const int h = wunit % a.nkvh;
     int b, block, group_base;
-    if (!locate(a, wunit / a.nkvh, true, b, block, group_base)) return;
+    if (!locate<GEO>(a, wunit / a.nkvh, true, b, block, group_base)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     block = __builtin_amdgcn_readfirstlane(block);
     group_base = __builtin_amdgcn_readfirstlane(group_base);
     TileGeom t;
-    if (!blockGeom(a, b, block, a.pps, t, split == 0 && wave == 0)) return;
+    if (!blockGeom<GEO>(a, b, block, a.pps, t, split == 0 && wave == 0)) return;
     // The geometry is wave-uniform: scalar registers, scalar branches.
     t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
     t.Lq = __builtin_amdgcn_readfirstlane(t.Lq);
     t.ctx = __builtin_amdgcn_readfirstlane(t.ctx);
     t.npages = __builtin_amdgcn_readfirstlane(t.npages);
-    prefillItem<OUT_F32, false, KV>(a, kvs, b, block, group_base, h, split, a.pps, __builtin_amdgcn_readfirstlane(groupsOf(a, b)),
+    prefillOne<OUT_F32, false, KV, GEO>(a, kvs, b, block, group_base, h, split, a.pps, __builtin_amdgcn_readfirstlane(groupsOf<GEO>(a, b)),
                          t);
 }
 
@@ -439,7 +678,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 // during this item); wave 0 writes the row. The decode kernel's math with
 // kWaves partial states instead of per-wave records.
 constexpr int kDecWindow = 64; // pairs per block-id window (one per lane)
-template <bool OUT_F32, class KV>
+template <bool OUT_F32, class KV, class GEO>
 __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, int h, int row, int c) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
@@ -448,7 +687,7 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
     const int G = a.G;
     const int np = (c + 15) >> 4;
     const int npr = (np + 1) >> 1;
-    const int p0 = wave * npr / kWaves, p1 = (wave + 1) * npr / kWaves;
+    const int p0 = wave * npr / GEO::kWaves, p1 = (wave + 1) * npr / GEO::kWaves;
     Acc acc;
     acc.reset();
     bool bad_block = false;
@@ -507,7 +746,7 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
     float lt = acc.l + __shfl_xor(acc.l, 16);
     lt += __shfl_xor(lt, 32);
     f32x4 *part_o = reinterpret_cast<f32x4 *>(&kvs[0][0]);                 // [kWaves - 1][8][64]
-    float *part_ml = reinterpret_cast<float *>(part_o + (kWaves - 1) * 8 * 64); // [kWaves - 1][2][64]
+    float *part_ml = reinterpret_cast<float *>(part_o + (GEO::kWaves - 1) * 8 * 64); // [kWaves - 1][2][64]
     if (wave > 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) part_o[((wave - 1) * 8 + i) * 64 + lane] = acc.o[i];
@@ -517,7 +756,7 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
     __syncthreads();
     if (wave == 0 && n < G) {
         float M = acc.m, L = lt;
-        for (int v = 0; v < kWaves - 1; ++v) {
+        for (int v = 0; v < GEO::kWaves - 1; ++v) {
             const float mv = part_ml[(v * 2 + 0) * 64 + lane];
             if (mv == -INFINITY) continue;
             const float Mn = fmaxf(M, mv);
@@ -538,10 +777,11 @@ __device__ __forceinline__ void decodeItem(const Args &a, StageBuf &kvs, int b, 
 // Exclusive prefix sums of va[0..n) and vb[0..n) in place (n <= 64 * 64), in
 // one pass by the whole workgroup; the totals go to *total_a and *total_b.
 // tmp: 130 ints of LDS. Barriers inside.
+template <class GEO>
 __device__ void blockExclusiveScan2(int *va, int *vb, int n, int *tmp, int *total_a, int *total_b) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nch = (n + 63) >> 6;
-    for (int ch = wave; ch < 2 * nch; ch += kWaves) {
+    for (int ch = wave; ch < 2 * nch; ch += GEO::kWaves) {
         const int which = ch >= nch ? 1 : 0, c = ch - which * nch;
         int *v = which ? vb : va;
         const int i = c * 64 + lane;
@@ -559,7 +799,7 @@ __device__ void blockExclusiveScan2(int *va, int *vb, int n, int *tmp, int *tota
         if (lane == 63) t[64] = incl;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 64 * kWaves) {
+    for (int i = threadIdx.x; i < n; i += 64 * GEO::kWaves) {
         va[i] += tmp[i >> 6];
         vb[i] += tmp[65 + (i >> 6)];
     }
@@ -609,14 +849,14 @@ __host__ __device__ constexpr size_t queueTableInts(int B, int units) {
     return size_t(6) * (B + 1) + size_t(4) * (units + 1);
 }
 
-template <bool OUT_F32, bool WITH_DECODE, bool CHOOSE, class KV>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <bool OUT_F32, bool WITH_DECODE, bool CHOOSE, class KV, class GEO>
+__global__ void __launch_bounds__(64 * GEO::kWaves) __attribute__((amdgpu_waves_per_eu(GEO::kWaves / 4, GEO::kWaves / 4)))
     prefillQueueKernel(Args a) {
     __shared__ StageBuf kvs;
     __shared__ int scan_tmp[2 * 65];
     __shared__ int s_item[2];
     extern __shared__ int tables[];
-    const int B = a.B, tid = threadIdx.x, nthreads = 64 * kWaves;
+    const int B = a.B, tid = threadIdx.x, nthreads = 64 * GEO::kWaves;
     int *cu = tables, *ctx = cu + (B + 1), *ubase = ctx + (B + 1), *gbase = ubase + (B + 1);
     int *nspl = gbase + (B + 1), *fpre = nspl + (a.block_units + 1), *ppos = fpre + (a.block_units + 1);
     int *punit = ppos + (a.block_units + 1), *dkey = punit + (a.block_units + 1), *dseq = dkey + (B + 1);
@@ -631,10 +871,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         int ng = 0;
         if (b < B) {
             const int lq = cu[b + 1] - cu[b];
-            ng = lq >= 2 ? (((lq * a.G + 15) >> 4) + kTiles - 1) / kTiles : 0;
+            ng = lq >= 2 ? (((lq * a.G + 15) >> 4) + GEO::kTiles - 1) / GEO::kTiles : 0;
         }
         gbase[b] = ng;
-        ubase[b] = (ng + kWaves - 1) / kWaves * a.nkvh;
+        ubase[b] = (ng + GEO::kWaves - 1) / GEO::kWaves * a.nkvh;
         // Single-query sequences (with_decode) with a valid query row and
         // length are decode items (nkvh each; else error bit 2, no items):
         // key = their length, -1 for the rest.
@@ -651,7 +891,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     }
     __syncthreads();
     int U = 0, n_groups = 0;
-    blockExclusiveScan2(gbase, ubase, B + 1, scan_tmp, &n_groups, &U);
+    blockExclusiveScan2<GEO>(gbase, ubase, B + 1, scan_tmp, &n_groups, &U);
     U = min(U, a.block_units);
     // Decode sequences longest first: dseq[rank] = b, the rank of b being
     // the number of valid sequences with a longer context, or as long and
@@ -674,7 +914,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             if constexpr (CHOOSE) dec_pages += ko[r] >= 0 ? (ko[r] + 15) >> 4 : 0;
         }
         if constexpr (CHOOSE) dec_pages = __builtin_amdgcn_readlane(waveInclusiveSum(dec_pages), 63);
-        for (int b = wave; b < B; b += kWaves) {
+        for (int b = wave; b < B; b += GEO::kWaves) {
             int kb = ko[0];
 #pragma unroll
             for (int r = 1; r < kRegs; ++r)
@@ -707,7 +947,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             if (q0 < 0 || q0 + lq > a.T || c > a.max_pages * 16 || lq > c) {
                 if (blockIdx.x == 0 && u == ubase[b]) atomicOr(a.err, kErrTooLong);
             } else {
-                const int qi_max = min(lq - 1, ((j + 1) * kWaves * kTiles * 16 - 1) / a.G);
+                const int qi_max = min(lq - 1, ((j + 1) * GEO::kColumns - 1) / a.G);
                 np = (c - lq + qi_max + 1 + 15) >> 4;
             }
         }
@@ -750,7 +990,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         __syncthreads();
     }
     int n_full = 0, n_part = 0;
-    blockExclusiveScan2(fpre, ppos, U + 1, scan_tmp, &n_full, &n_part);
+    blockExclusiveScan2<GEO>(fpre, ppos, U + 1, scan_tmp, &n_full, &n_part);
     for (int u = tid; u < U; u += nthreads)
         if (nspl[u] > fpre[u + 1] - fpre[u]) punit[ppos[u]] = u;
     __syncthreads();
@@ -784,17 +1024,17 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             t.q0 = __builtin_amdgcn_readfirstlane(cu[b]);
             t.Lq = __builtin_amdgcn_readfirstlane(cu[b + 1]) - t.q0;
             t.ctx = __builtin_amdgcn_readfirstlane(ctx[b]);
-            const int qi_max = min(t.Lq - 1, ((block + 1) * kWaves * kTiles * 16 - 1) / a.G);
+            const int qi_max = min(t.Lq - 1, ((block + 1) * GEO::kColumns - 1) / a.G);
             t.npages = (t.ctx - t.Lq + qi_max + 1 + 15) >> 4;
             t.nsplit = __builtin_amdgcn_readfirstlane(nspl[u]);
             const int group_base = __builtin_amdgcn_readfirstlane(gbase[b]);
             const int groups_b = __builtin_amdgcn_readfirstlane(gbase[b + 1]) - group_base;
-            prefillItem<OUT_F32, CHOOSE, KV>(a, kvs, b, block, group_base, h, split, pps, groups_b, t);
+            prefillOne<OUT_F32, CHOOSE, KV, GEO>(a, kvs, b, block, group_base, h, split, pps, groups_b, t);
         } else if constexpr (WITH_DECODE) {
             const int d = item - n_full;
             const int b = __builtin_amdgcn_readfirstlane(dseq[d / a.nkvh]);
             const int h = d - (d / a.nkvh) * a.nkvh;
-            decodeItem<OUT_F32, KV>(a, kvs, b, h, __builtin_amdgcn_readfirstlane(cu[b]),
+            decodeItem<OUT_F32, KV, GEO>(a, kvs, b, h, __builtin_amdgcn_readfirstlane(cu[b]),
                                 __builtin_amdgcn_readfirstlane(ctx[b]));
         }
     }
@@ -807,12 +1047,12 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 // Merge the split records of each unit with more than one split.
 constexpr int kMergeBatch = 4;
 
-template <bool OUT_F32, bool CHOOSE> __global__ void __launch_bounds__(64) prefillCombineKernel(Args a) {
+template <bool OUT_F32, bool CHOOSE, class GEO> __global__ void __launch_bounds__(64) prefillCombineKernel(Args a) {
     const int lane = threadIdx.x;
     const int n = lane & 15;
     const int grp = lane >> 4;
-    const int unit = blockIdx.x / kTiles;
-    const int k = blockIdx.x - unit * kTiles; // tile of the group this wave merges
+    const int unit = blockIdx.x / GEO::kTiles;
+    const int k = blockIdx.x - unit * GEO::kTiles; // tile of the group this wave merges
     if (unit >= a.units) return;
     const int h = unit % a.nkvh;
     // The split size prefillQueueKernel chose: requested here, by a vector
@@ -825,17 +1065,17 @@ template <bool OUT_F32, bool CHOOSE> __global__ void __launch_bounds__(64) prefi
         pps = a.queue[at];
     }
     int b, group, group_base;
-    if (!locate(a, unit / a.nkvh, false, b, group, group_base)) return;
+    if (!locate<GEO>(a, unit / a.nkvh, false, b, group, group_base)) return;
     pps = __builtin_amdgcn_readfirstlane(pps);
     TileGeom t;
-    if (!blockGeom(a, b, group / kWaves, pps, t, false) || t.nsplit <= 1) return;
+    if (!blockGeom<GEO>(a, b, group / GEO::kWaves, pps, t, false) || t.nsplit <= 1) return;
     const int G = a.G;
-    const int pair = (group * kTiles + k) * 16 + n;
+    const int pair = (group * GEO::kTiles + k) * 16 + n;
     const int qi = pair / G;
     const int g = pair - qi * G;
     const bool col_ok = qi < t.Lq;
     const int c = k * 16 + n;
-    const float *recs = a.records + size_t(unit) * splitStride<CHOOSE>(a, pps) * kRecordFloats;
+    const float *recs = a.records + size_t(unit) * splitStride<CHOOSE>(a, pps) * GEO::kRecordFloats;
     float M = -INFINITY, L = 0.f;
     f32x4 o[8];
 #pragma unroll
@@ -847,12 +1087,12 @@ template <bool OUT_F32, bool CHOOSE> __global__ void __launch_bounds__(64) prefi
             f32x4 orr[kMergeBatch][8];
 #pragma unroll
             for (int s = 0; s < kMergeBatch; ++s) {
-                const float *rec = recs + size_t(min(k0 + s, t.nsplit - 1)) * kRecordFloats;
-                const float2 ml = *reinterpret_cast<const float2 *>(rec + kTiles * 16 * kHeadDim + 2 * c);
+                const float *rec = recs + size_t(min(k0 + s, t.nsplit - 1)) * GEO::kRecordFloats;
+                const float2 ml = *reinterpret_cast<const float2 *>(rec + GEO::kTiles * 16 * kHeadDim + 2 * c);
                 mr[s] = k0 + s < t.nsplit ? ml.x : -INFINITY;
                 lr[s] = ml.y;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) orr[s][i] = loadRecordO<RECORDS_F32>(rec, (i * kTiles * 16 + c) * 16 + grp * 4);
+                for (int i = 0; i < 8; ++i) orr[s][i] = loadRecordO<RECORDS_F32>(rec, (i * GEO::kTiles * 16 + c) * 16 + grp * 4);
             }
 #pragma unroll
             for (int s = 0; s < kMergeBatch; ++s) {
@@ -908,8 +1148,11 @@ static bool queueFits(int B, const PagedAttentionPlan &plan) {
            queueTableInts(B, plan.block_units) * sizeof(int) <= kQueueTableBytes;
 }
 
-PagedAttentionPlan planPrefill(int B, int T, int nkvh, int group, int max_pages) {
+PagedAttentionPlan planPrefill(int B, int T, int nkvh, int group, int max_pages, bool f8) {
     PagedAttentionPlan p{};
+    const int kTiles = f8 ? GeoF8::kTiles : GeoBf16::kTiles, kWaves = f8 ? GeoF8::kWaves : GeoBf16::kWaves;
+    const int kColumns = f8 ? GeoF8::kColumns : GeoBf16::kColumns;
+    const size_t kRecordFloats = f8 ? GeoF8::kRecordFloats : GeoBf16::kRecordFloats;
     const int groups = ((T * group + 15) / 16 + kTiles - 1) / kTiles + B; // upper bound over the batch
     p.units = groups * nkvh;
     p.units_padded = p.units;
@@ -936,7 +1179,7 @@ PagedAttentionPlan planPrefill(int B, int T, int nkvh, int group, int max_pages)
     // pages four of 530 29.2 / 33.3).
     p.pages_per_split_min = pps;
     p.max_splits = std::max(1, (max_pages + pps - 1) / pps);
-    const long long blocks = ((long long)T * group + kWaves * kTiles * 16 - 1) / (kWaves * kTiles * 16) * nkvh;
+    const long long blocks = ((long long)T * group + kColumns - 1) / kColumns * nkvh;
     const bool long_ones = T >= 512LL * B;
     const bool pays = max_pages > 64 ? (B == 1 || long_ones) && blocks * max_pages < 48LL * cuCount()
                                      : long_ones && 2 * blocks <= cuCount() && (B == 1 || max_pages > 40);
@@ -999,7 +1242,7 @@ void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_
     a.block_units = plan.block_units;
     a.block_units_padded = plan.block_units_padded;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const dim3 grid(plan.block_units_padded * a.max_splits), block(64 * kWaves), cblock(64);
+    const dim3 grid(plan.block_units_padded * a.max_splits), block(64 * (k_scale ? GeoF8::kWaves : GeoBf16::kWaves)), cblock(64);
     auto s = static_cast<hipStream_t>(stream);
     // The persistent kernel whenever its item tables fit in LDS beside the
     // stages (and a counter buffer is given); otherwise one workgroup per
@@ -1012,21 +1255,21 @@ void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_
     auto launchOver = [&](auto f32, auto chosen, auto kv) {
         constexpr bool F32 = decltype(f32)::value, CHOOSE = decltype(chosen)::value;
         using KV = decltype(kv);
+        using GEO = std::conditional_t<KV::kScaled, GeoF8, GeoBf16>;
         if (queued && a.with_decode)
-            hipLaunchKernelGGL((prefillQueueKernel<F32, true, CHOOSE, KV>), qgrid, block, unsigned(table_bytes), s, a);
+            hipLaunchKernelGGL((prefillQueueKernel<F32, true, CHOOSE, KV, GEO>), qgrid, block, unsigned(table_bytes), s, a);
         else if (queued)
-            hipLaunchKernelGGL((prefillQueueKernel<F32, false, CHOOSE, KV>), qgrid, block, unsigned(table_bytes), s, a);
+            hipLaunchKernelGGL((prefillQueueKernel<F32, false, CHOOSE, KV, GEO>), qgrid, block, unsigned(table_bytes), s, a);
         else
-            hipLaunchKernelGGL((prefillKernel<F32, KV>), grid, block, 0, s, a);
+            hipLaunchKernelGGL((prefillKernel<F32, KV, GEO>), grid, block, 0, s, a);
+        if (a.max_splits > 1)
+            hipLaunchKernelGGL((prefillCombineKernel<F32, CHOOSE, GEO>), dim3(plan.units * GEO::kTiles), cblock, 0, s, a);
     };
     auto launch = [&](auto f32, auto chosen) {
-        constexpr bool F32 = decltype(f32)::value, CHOOSE = decltype(chosen)::value;
         if (k_scale)
             launchOver(f32, chosen, KvF8());
         else
             launchOver(f32, chosen, KvBf16());
-        if (a.max_splits > 1)
-            hipLaunchKernelGGL((prefillCombineKernel<F32, CHOOSE>), dim3(plan.units * kTiles), cblock, 0, s, a);
     };
     if (out_f32) {
         if (choose) launch(std::true_type(), std::true_type());

@@ -5,6 +5,7 @@
 #include "cpu/cpu_kernels.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace llaisys::ops {
 
@@ -365,7 +366,7 @@ void attendOnDevice(const char *op, const tensor_t &out, const tensor_t &q, cons
                   op << ": at most " << K::kDecodeMaxBatch << " sequences per varlen call");
     const auto *cu = reinterpret_cast<const int32_t *>(cu_q->data());
     auto dplan = K::planDecode(int(B), int(nkvh), G, max_pages, ks != nullptr);
-    auto pplan = K::planPrefill(int(B), int(T), int(nkvh), G, max_pages);
+    auto pplan = K::planPrefill(int(B), int(T), int(nkvh), G, max_pages, ks != nullptr);
     float *records = static_cast<float *>(rt.scratch(std::max(dplan.record_bytes, pplan.partial_bytes)));
     int *queue = rt.queueCounters();
     // The persistent prefill kernel takes the single-query sequences too
@@ -575,6 +576,7 @@ void pagedAttentionF8(const tensor_t &out, const tensor_t &q, const tensor_t &k_
     const int max_pages = int(block_table->shape()[1]);
     LLAISYS_CHECK(max_pages > 0, op << ": block_table has no pages");
     LLAISYS_CHECK(k_pool->shape()[0] > 0, op << ": the pool has no blocks");
+    LLAISYS_CHECK(scale > 0.f && std::isfinite(scale), op << ": scale must be positive and finite, got " << scale);
     if (!host)
         return attendOnDevice(op, out, q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_len, cu_q, scale, false);
     C::pagedAttentionF8(out->data(), out->dtype() == LLAISYS_DTYPE_F32, reinterpret_cast<const uint16_t *>(q->data()),

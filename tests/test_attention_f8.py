@@ -202,5 +202,10 @@ def test_refusals():
         L.Ops.paged_attention_varlen_f8(out, q, *pools, table, ctx, ctx, 0.1)
     with pytest.raises(L.LlaisysError, match="out"):
         L.Ops.paged_attention_varlen_f8(cu, q, *pools, table, cu, ctx, 0.1)
+    for scale in (0.0, -0.1, float("nan"), float("inf")):
+        with pytest.raises(L.LlaisysError, match="scale must be positive"):
+            L.Ops.paged_attention_f8(out, q, *pools, table, ctx, scale)
+        with pytest.raises(L.LlaisysError, match="scale must be positive"):
+            L.Ops.paged_attention_varlen_f8(out, q, *pools, table, cu, ctx, scale)
     with pytest.raises(L.LlaisysError, match="f8"):  # an 8-bit pool to the bf16 entry point
         L.Ops.paged_attention(out, q, pools[0], pools[1], table, ctx, 0.1)
