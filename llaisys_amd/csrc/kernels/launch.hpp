@@ -160,6 +160,18 @@ void pagedPrefill(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_
                   float *records, int *err, int *queue, void *stream, const float *k_scale = nullptr,
                   const float *v_scale = nullptr);
 
+// ---- varlen attention over the 8-bit pages in one launch (paged_units.hip)
+// Chunks and single queries alike. unitShape: tiles of 16 columns and waves of a
+// workgroup for this batch; no tiles: it is left to pagedDecode and pagedPrefill.
+struct UnitShape {
+    int tiles, waves;
+};
+UnitShape unitShape(int B, int T, int nkvh, int group, int max_pages);
+void pagedVarlenUnits(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,
+                      const float *k_scale, const float *v_scale, const int32_t *block_table, const int32_t *ctx_len,
+                      const int32_t *cu_q, int B, int T, int nh, int nkvh, int max_pages, int num_blocks, float scale,
+                      UnitShape shape, int *err, void *stream);
+
 // ---- a step's tables (paged_map.hip)
 // Per sequence its c = ctx_len and n = new_len: cu_new the prefix sums of n (at
 // most T), pages [ceil(c / 16), ceil((c + n) / 16)) of block_table from

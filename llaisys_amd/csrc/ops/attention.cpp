@@ -365,6 +365,11 @@ void attendOnDevice(const char *op, const tensor_t &out, const tensor_t &q, cons
     LLAISYS_CHECK(B <= size_t(K::kDecodeMaxBatch),
                   op << ": at most " << K::kDecodeMaxBatch << " sequences per varlen call");
     const auto *cu = reinterpret_cast<const int32_t *>(cu_q->data());
+    if (const auto shape = ks ? K::unitShape(int(B), int(T), int(nkvh), G, max_pages) : K::UnitShape{}; shape.tiles) {
+        K::pagedVarlenUnits(out->data(), f32, qp, kp, vp, ks, vs, tab, ctx, cu, int(B), int(T), int(nh), int(nkvh),
+                            max_pages, nb, scale, shape, rt.errorWord(), rt.stream());
+        return;
+    }
     auto dplan = K::planDecode(int(B), int(nkvh), G, max_pages, ks != nullptr);
     auto pplan = K::planPrefill(int(B), int(T), int(nkvh), G, max_pages, ks != nullptr);
     float *records = static_cast<float *>(rt.scratch(std::max(dplan.record_bytes, pplan.partial_bytes)));

@@ -42,6 +42,8 @@ def want_of(cache, table, lens, qn, q):
     K, V = cache.values(0), cache.values(1)
     out, most, r = [], 0.0, 0
     for b, (n, c) in enumerate(zip(qn, lens)):
+        if n == 0:
+            continue
         at = table[b, :-(-c // 16)]
         rows = lambda x: x[at].transpose(0, 2, 1, 3).reshape(-1, x.shape[1], 128)[:c]  # noqa: E731
         o, m = attend64(f64(q[r:r + n]), rows(K), rows(V), SCALE)
@@ -135,6 +137,43 @@ def test_chunks_long_and_many(dtype, qn, prior, extra):
     assert L.device_error_flags() == 0
     want, most = want_of(cache, table, lens, qn, q)
     check(got, want, most, cache, dtype, max(lens), True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("qn, prior, pages", [
+    # on both sides of the lines between the kernels: 256 and 258 blocks of queries, 900 and 902
+    ([338], [0], 0), ([341], [0], 0), ([1197], [0], 0), ([1200], [0], 0), ([1100] + [1] * 90, [40] + [300] * 90, 0),
+    # tables of 256 and 257 pages with 528 blocks, of 300 with 512 and 516, of 512 and 513 with few
+    ([700], [3396], 256), ([700], [3397], 257), ([680], [33], 300), ([683], [33], 300), ([64], [8128], 512),
+    ([64], [8129], 513), ([2, 1, 1, 70], [0, 0, 8191, 4000], 512),
+    # sequences without queries among the others
+    ([0, 20, 0, 0, 1, 0], [9, 40, 0, 70, 8, 1], 0),
+])
+def test_chunks_at_the_lines(dtype, qn, prior, pages):
+    lens = [a + b for a, b in zip(qn, prior)]
+    cache, table, q = case(19, lens, 12, 2, qn, extra_pages=max(0, pages - -(-max(lens) // 16)), stale_nan=True)
+    assert pages in (0, table.shape[1])
+    cu = np.concatenate([[0], np.cumsum(qn)])
+    got = varlen("amd", cache, table, q, cu, lens, dtype)
+    assert L.device_error_flags() == 0
+    want, most = want_of(cache, table, lens, qn, q)
+    check(got, want, most, cache, dtype, max(lens), True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [[60, 19, 33], [60, 1000, 33], [60, 0, 33]])  # too short, past the table, none
+@pytest.mark.parametrize("pages", [0, 600])
+def test_a_bad_sequence_leaves_the_others(device, bad, pages):
+    qn, lens = [40, 20, 33], [60, 20, 33]
+    cache, table, q = case(23, lens, 12, 2, qn, extra_pages=pages if device == "amd" else 0)
+    cu = np.concatenate([[0], np.cumsum(qn)])
+    ctx = bad if table.shape[1] * 16 < 1000 or 1000 not in bad else [60, 100000, 33]
+    got = varlen(device, cache, table, q, cu, ctx, torch.bfloat16)
+    assert L.device_error_flags() == TOO_LONG
+    want, most = want_of(cache, table, lens, qn, q)
+    good = np.r_[0:40, 60:93]
+    check(got[good], want[good], most, cache, torch.bfloat16, 60, True)
 
 
 @pytest.mark.parametrize("device", DEVICES)
