@@ -86,10 +86,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 #pragma unroll
         for (int e = 0; e < EL; ++e) top = max(top, __float_as_uint(float(r.e[e])) & 0x7fffffffu);
     };
-    Piece held[kPieces];
+    Piece held[kPieces] = {};
+    if (pieces > 0) { // (past the row its last piece again)
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) held[i] = load(max(0, min(tid + i * THREADS, pieces - 1)));
-    if (pieces > 0) {
+        for (int i = 0; i < kPieces; ++i) held[i] = load(min(tid + i * THREADS, pieces - 1));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) search(held[i]);
     }

@@ -75,6 +75,11 @@ void checkPool(const tensor_t &kp, const tensor_t &vp, const char *op) {
     LLAISYS_CHECK(kp->shape()[0] < size_t(1) << 31, op << ": too many blocks");
 }
 
+// Rows and pages of the 8-bit ops move in 16 B pieces.
+void requireAligned(const tensor_t &t, const char *op, const char *name) {
+    LLAISYS_CHECK(reinterpret_cast<uintptr_t>(t->data()) % 16 == 0, op << ": " << name << " must begin on a 16 B boundary");
+}
+
 // The 8-bit pools: F8 of the same shape, with F32 scales [num_blocks, nkvh].
 void checkPoolF8(const tensor_t &kp, const tensor_t &vp, const tensor_t &ks, const tensor_t &vs, const char *op) {
     for (auto *t : {&kp, &vp}) {
@@ -83,6 +88,7 @@ void checkPoolF8(const tensor_t &kp, const tensor_t &vp, const tensor_t &ks, con
                       op << ": pool must be [num_blocks, nkvh, 16, 128], got " << shapeStr(*t));
         requireDtype(*t, LLAISYS_DTYPE_F8, op, "pool");
         requireContiguous(*t, op, "pool");
+        requireAligned(*t, op, "pool");
     }
     LLAISYS_CHECK(kp->shape() == vp->shape(), op << ": K and V pools differ in shape");
     LLAISYS_CHECK(kp->shape()[0] < size_t(1) << 31, op << ": too many blocks");
@@ -486,6 +492,7 @@ void pagedKVAppendF8(const tensor_t &k_pool, const tensor_t &v_pool, const tenso
     for (const auto *t : {&k_new, &v_new}) {
         requireDtype(*t, LLAISYS_DTYPE_BF16, op, "k_new and v_new");
         requireContiguous(*t, op, "k_new and v_new");
+        requireAligned(*t, op, "k_new and v_new");
     }
     const size_t T = k_new->shape()[0];
     requireShape(slots, {T}, op, "slots");
@@ -522,6 +529,7 @@ void pagedKVGatherF8(const tensor_t &k_out, const tensor_t &v_out, const tensor_
     for (const auto *t : {&k_out, &v_out}) {
         requireDtype(*t, LLAISYS_DTYPE_BF16, op, "k_out and v_out");
         requireContiguous(*t, op, "k_out and v_out");
+        requireAligned(*t, op, "k_out and v_out");
     }
     LLAISYS_CHECK(cu_seqlens->ndim() == 1 && cu_seqlens->shape()[0] >= 1, op << ": cu_seqlens must be [B+1]");
     const size_t B = cu_seqlens->shape()[0] - 1;
@@ -581,6 +589,8 @@ void pagedAttentionF8(const tensor_t &out, const tensor_t &q, const tensor_t &k_
     const int max_pages = int(block_table->shape()[1]);
     LLAISYS_CHECK(max_pages > 0, op << ": block_table has no pages");
     LLAISYS_CHECK(k_pool->shape()[0] > 0, op << ": the pool has no blocks");
+    requireAligned(q, op, "q");
+    requireAligned(out, op, "out");
     LLAISYS_CHECK(scale > 0.f && std::isfinite(scale), op << ": scale must be positive and finite, got " << scale);
     if (!host)
         return attendOnDevice(op, out, q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_len, cu_q, scale, false);

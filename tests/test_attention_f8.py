@@ -95,7 +95,7 @@ def test_decode(device, dtype, nh, nkvh, lens):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lens, extra", [
     ([2000], 0), ([700], 60), ([9000, 3], 0), (list(range(600, 1024, 7)), 0), (list(range(1, 8192, 177)), 10),
-    ([1] * 200, 3), (list(range(1, 300)), 100),
+    ([1] * 200, 3), (list(range(1, 300)), 100), ([1 + i % 37 for i in range(4100)], 0),  # more than a launch takes
     # on both sides of the lines between the kernels: tables of 48 and 49, 80 and 81, 96 and 97, 128 and 129 pages
     ([768, 5], 0), ([769, 5], 0), ([1280] + [1] * 9, 0), ([1281] + [1] * 9, 0), ([1536] + [70] * 31, 0),
     ([1537] + [70] * 31, 0), ([2048] + [33] * 63, 0), ([2049] + [33] * 63, 0),
@@ -246,5 +246,9 @@ def test_refusals():
             L.Ops.paged_attention_f8(out, q, *pools, table, ctx, scale)
         with pytest.raises(L.LlaisysError, match="scale must be positive"):
             L.Ops.paged_attention_varlen_f8(out, q, *pools, table, cu, ctx, scale)
+    odd = give(torch.zeros(2 * 12 * 128 + 4, dtype=torch.bfloat16), dev).slice(0, 4, 2 * 12 * 128 + 4).view(2, 12, 128)
+    for args in ((out, odd), (odd, q)):
+        with pytest.raises(L.LlaisysError, match="16 B boundary"):
+            L.Ops.paged_attention_f8(*args, *pools, table, ctx, 0.1)
     with pytest.raises(L.LlaisysError, match="f8"):  # an 8-bit pool to the bf16 entry point
         L.Ops.paged_attention(out, q, pools[0], pools[1], table, ctx, 0.1)

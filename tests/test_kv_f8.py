@@ -253,5 +253,14 @@ def test_refusals():
     with pytest.raises(L.LlaisysError, match="contiguous"):
         flat = give(torch.zeros(4, 128, 2, dtype=torch.bfloat16), dev).permute(0, 2, 1)
         L.Ops.paged_kv_append_f8(*pools, flat, flat, sl)
+    flat = give(torch.zeros(4 * 256 + 4, dtype=torch.bfloat16), dev).slice(0, 4, 4 * 256 + 4).view(4, 2, 128)
+    for rows in ((flat, kn), (kn, flat)):
+        with pytest.raises(L.LlaisysError, match="16 B boundary"):
+            L.Ops.paged_kv_append_f8(*pools, *rows, sl)
+        with pytest.raises(L.LlaisysError, match="16 B boundary"):
+            L.Ops.paged_kv_gather_f8(*rows, *pools, table, cu)
+    with pytest.raises(L.LlaisysError, match="16 B boundary"):
+        bytes_ = give(torch.zeros(3 * 2 * 2048 + 8, dtype=torch.uint8), dev).slice(0, 8, 3 * 2 * 2048 + 8)
+        L.Ops.paged_kv_append_f8(pools[0], bytes_.view(3, 2, 16, 128), *pools[2:], kn, kn, sl)
     with pytest.raises(L.LlaisysError, match="pairs"):
         L.Ops.paged_kv_copy_blocks_f8(*pools, cu)
