@@ -84,6 +84,40 @@ def test_rows_on_both_sides_of_one_launch(device, extra):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [512, 513, 1024, 1025, 4096, 4097, 9000])
+@pytest.mark.parametrize("B", [1, 5, 1024, 1025])
+@pytest.mark.parametrize("how", ["list", "in place", "no list", "no reach"])
+def test_rows_spread_over_workgroups(device, T, B, how):
+    """Ragged batches that fill T rows but for a few; with a list that ends early; mapped by the host."""
+    r = np.random.RandomState(T + B)
+    new = r.multinomial(T - 3 if T > B else T // 2, np.full(B, 1 / B) if B > 5 else r.dirichlet(np.ones(B)))
+    ctx = r.randint(0, 200, B)
+    width = int((ctx + new).max()) // 16 + 2
+    table, free = mapped(T, ctx + new if how == "no list" else ctx, width, int((new // 16 + 2).sum()))
+    if how == "no list":
+        check(device, table, ctx, new, T)
+    else:
+        check(device, table, ctx, new, T, free[:len(free) // 4] if how == "no reach" else free, in_place=how == "in place")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [500, 600])
+def test_blocks_that_are_negative(device, T):
+    """In the list, in the table; at a sequence's first page or a later one."""
+    ctx, new = [0, 20, 16, 5, 31], [100, 90, 64, 0, 200]
+    for at in (0, 3, 9, 12, 17):
+        table, free = mapped(9, ctx, 20, 40)
+        free[at] = -5
+        check(device, table, ctx, new, T, free)
+    table, free = mapped(9, ctx, 20, 40)
+    table[1, 1] = -1
+    check(device, table, ctx, new, T, free)
+    full, _ = mapped(9, [c + n for c, n in zip(ctx, new)], 20, 3)
+    full[0, 4] = full[4, 2] = full[1, 1] = -3
+    check(device, full, ctx, new, T)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_tables_that_the_host_mapped(device):
     ctx, new = [0, 15, 16, 30], [5, 2, 16, 40]
     table, _ = mapped(3, [c + n for c, n in zip(ctx, new)], 6, 2)
