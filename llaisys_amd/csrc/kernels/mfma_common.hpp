@@ -175,14 +175,14 @@ __device__ __forceinline__ void softmaxUpdate(Acc &acc, const float (&sv)[NP][8]
     for (int j = 0; j < NP; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) mloc = fmaxf(mloc, sv[j][i]);
-    mloc = maxOverGroups(mloc);
     // Lazy rescale: a column keeps its running max until a score exceeds it
     // by more than 2^kLazyLog2 (P then stays below that bound). Only when some
     // column of the wave crosses it do all columns move to their true max and
-    // rescale O and l; the normalised result is the same either way.
+    // rescale O and l; the normalised result is the same either way. Until then
+    // each lane compares its own scores, not its column's.
     constexpr float kLazyLog2 = 8.f;
-    const float m_true = fmaxf(acc.m, mloc * scale_log2);
-    if (__builtin_amdgcn_ballot_w64(m_true > acc.m + kLazyLog2) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mloc * scale_log2 > acc.m + kLazyLog2) != 0) {
+        const float m_true = fmaxf(acc.m, maxOverGroups(mloc) * scale_log2);
         const float alpha = exp2Fast(acc.m - ((m_true == -INFINITY) ? 0.f : m_true));
         acc.l *= alpha;
 #pragma unroll

@@ -11,12 +11,19 @@
 // for each other at, no partial records and no second launch; the persistent
 // kernel spends some 20 us on those. The price is that every block reads its
 // pages from L2 again and widens them for TILES tiles only (8 TILES in the
-// persistent kernel), so batches of much work go there (unitShape).
+// persistent kernel), so wide tables go there (unitShape).
 //
-// What bounds it is a wave's chain of load, widen, QK, softmax, PV per page
-// pair with two waves on a SIMD: one chunk of 777 queries 12.8 us (persistent
-// kernel 27.5), 6 chunks of 340 after 1700 tokens 38.9 us (50.4), where the
-// matrix instructions alone would take 14 us.
+// What bounds it is the vector unit: widening, exponentials (128 of a tile's
+// some 400 cycles per page pair) and rounding beside 256 cycles of matrix
+// instructions, on two waves a SIMD. 12 query and 2 kv heads, us, here and the
+// persistent kernel: a chunk of 777 queries 12.8, 27.5; 4 chunks of 512 after
+// 4096 tokens beside 60 single queries 68.4, 77.9.
+//
+// Consecutive workgroups take the kv heads in turn, as consecutive workgroups go
+// to the XCDs in turn: where the heads divide the 8 XCDs, an XCD's L2 holds the
+// pages of one head. Runs of two workgroups of a head and two of the next took 4
+// x 512 after 4096 from 68 to 84 us; longer runs of one head on an XCD gained
+// nothing (66-70).
 #include "mfma_common.hpp"
 
 #include "../device/hip_check.hpp"
@@ -78,7 +85,12 @@ __device__ bool placeOf(const UnitArgs &a, int index, int columns, Place &p) {
 
 template <bool OUT_F32, int TILES, int UW>
 __global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2, 2))) varlenUnitKernel(UnitArgs a) {
-    constexpr int NSTAGE = 2, PARTS = decodeParts<OUT_F32>(), COLS = 16 * TILES, WINDOW = 64;
+    // Parts of bf16 that a weight is summed in: 32-bit outputs hold 2^-24 of it,
+    // 16-bit ones of a tile 2^-16. Large batches with 16-bit outputs (TILES == 2)
+    // take one, 2^-9, which the output's own rounding is as large as: 3 chunks of
+    // 700 after 1500 tokens 42.1 -> 37.9 us.
+    constexpr int PARTS = OUT_F32 ? 3 : TILES == 2 ? 1 : 2;
+    constexpr int NSTAGE = 2, COLS = 16 * TILES, WINDOW = 64;
     __shared__ f32x4 part_o[UW / 2][8][64];
     __shared__ float part_ml[UW / 2][2][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -233,24 +245,26 @@ __global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2,
 } // namespace
 
 // By the number of workgroups that blocks of one tile make, at 12 query and 2 kv
-// heads (us: persistent kernel, then 1 tile and 4 waves, 1 and 8, 2 and 4):
+// heads (us: persistent kernel, then 1 tile and 4 waves, 1 and 8, 2 and 4, the
+// last still with two parts of a weight):
 //   up to 256: 64 after 1900 tokens 25.8, 15.1, 13.5, 21.9; 64 after 8000 39.2,
 //     45.6, 39.4, 67.1; 256 after 8000 45.3, 47.2, 39.3, 69.6; 333 alone 22.6,
 //     7.1, 7.2, 9.7: 8 waves, which halve the walk over a long context
 //   up to 900: 777 alone 27.5, 12.8, 18.0, 14.3; 2 x 256 and 60 single queries
 //     25.7, 20.0, 23.9, 28.2; 1200 alone (902) 34.8, 19.7, 28.1, 19.4
 //   more: 4 x 1000 44.7, 50.7, 80.7, 41.9; 6 x 340 after 1700 50.4, 44.1, 54.6,
-//     38.8; 700 after 1000 twice and 150 single ones 72.6, 67.5, 78.7, 68.9
+//     38.6; 700 after 1000 twice and 150 single ones 72.6, 67.5, 78.7, 68.9
 // A block's walk is as long as its context, which only the table's width bounds
-// here. At 4096 tokens the persistent kernel draws level with many blocks (4 x
-// 512 after 4096 and 60 single ones 77.9, 2 tiles 77.5) and leads beyond (6 x 340
-// after 4000 55.4 to 65.2); with blocks for at most two rounds of the CUs it does
-// so at 8192.
+// here, and the persistent kernel splits long ones. Up to 8192 tokens that
+// decides little (us, persistent and this: 2 x 2000 after 4000 130, 100; 8000
+// alone 273, 233; 4 x 1000 after 8000 173, 154; 8 x 512 after 8000 and 60 single
+// ones up to 8000 182, 211; 4 x 256 after 6000 and 60 67, 76); beyond, a few
+// queries after 16000 tokens walk alone for 80 us.
 // Three and four tiles a block need one wave on a SIMD: 6 x 340 after 1700 55.6
 // and 61.0.
 UnitShape unitShape(int B, int T, int nkvh, int group, int max_pages) {
+    if (max_pages > 512) return {0, 0};
     const long long blocks = (((long long)T * group + 15) / 16 + B) * nkvh;
-    if (max_pages > 512 || (max_pages > 256 && blocks > 512)) return {0, 0};
     return blocks <= 256 ? UnitShape{1, 8} : blocks <= 900 ? UnitShape{1, 4} : UnitShape{2, 4};
 }
 
