@@ -1262,7 +1262,12 @@ template <ElemType O> __global__ void __launch_bounds__(256) biasRowsI8Kernel(Ge
 
 // 8-bit operands move and multiply as 16-bit ones of half the K do (the same
 // bytes, and a 64-k step of them takes an MFMA the time of a 32-k one), so the
-// 16-bit plans and lines are theirs at K / 2.
+// 16-bit plans and lines are theirs at K / 2: over 22 shapes, every tile with 1
+// to 8 splits timed, they are within 5 % of the best one, but for 8192 x 1536 x
+// 8960 (98 us; 256 x 192 takes 90). us, 8 and 16 bits: 1 x 1536 x 8960 4.9, 7.3
+// (a few rows: W's bytes), 777 x 2048 x 1536 7.6, 13.0 (one round of 64 x 64
+// tiles: its fixed time), 8192 x 17920 x 1536 246 (1830 TOP/s of the 2063 that a
+// large product reaches), 383.
 bool tiledI8(const void *x, const void *w, int K) {
     return K % 16 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) % 16 == 0;
 }

@@ -988,6 +988,10 @@ DecodePlan planDecode(int B, int nkvh, int group, int max_pages, bool f8) {
     // batches (3.54 ms per step against 3.56-3.60 at 1.5 and 3.56 at 2 waves
     // per CU; 1 wave per CU was 3 % slower than 1.5), slightly ahead for the
     // mixed batch and neutral for the config-3 batch (53.15 us at 1.5 or 1.75).
+    // 8-bit pages: four per CU; half the bytes leave a wave longer at its own
+    // chain of widening, QK, softmax and PV (64 x 512-8192 tokens, combine
+    // included, at 1.75 / 2.5 / 3 / 4 / 5 / 6 / 8 per CU: 39.0, 34.0, 31.8, 32.0,
+    // 36.5, 36.3, 38.6 us; 142 MB, which a copy would move in 29).
     const int fill = std::max(1, envInt("LLAISYS_DECODE_WAVES", f8 ? computeUnits() * 4 : computeUnits() * 7 / 4));
     p.waves = int(std::max<long long>(fill, (max_pairs + kPairsPerWave - 1) / kPairsPerWave));
     p.record_bytes = size_t(2) * p.waves * group * (kHeadDim + 2) * sizeof(float);
