@@ -83,29 +83,16 @@ __device__ bool placeOf(const UnitArgs &a, int index, int columns, Place &p) {
     return false;
 }
 
-template <bool OUT_F32, int TILES, int UW>
-__global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2, 2))) varlenUnitKernel(UnitArgs a) {
-    // Parts of bf16 that a weight is summed in: 32-bit outputs hold 2^-24 of it,
-    // 16-bit ones of a tile 2^-16. Large batches with 16-bit outputs (TILES == 2)
-    // take one, 2^-9, which the output's own rounding is as large as: 3 chunks of
-    // 700 after 1500 tokens 42.1 -> 37.9 us.
-    constexpr int PARTS = OUT_F32 ? 3 : TILES == 2 ? 1 : 2;
+// The 16 TILES columns from col0 on, of kv head h.
+template <bool OUT_F32, int TILES, int UW, int PARTS>
+__device__ __forceinline__ void attendBlock(const UnitArgs &a, const Place &p, int h, int col0) {
     constexpr int NSTAGE = 2, COLS = 16 * TILES, WINDOW = 64;
     __shared__ f32x4 part_o[UW / 2][8][64];
     __shared__ float part_ml[UW / 2][2][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, n = lane & 15, grp = lane >> 4;
     const int G = a.G;
-    // Longest first: a sequence's last blocks see the most keys.
-    const int u = a.units - 1 - int(blockIdx.x);
-    const int h = u % a.nkvh;
-    Place p;
-    if (!placeOf(a, u / a.nkvh, COLS, p)) return;
-    if (!fits(p.q0, p.q0 + p.Lq, p.ctx, a)) {
-        if (threadIdx.x == 0) atomicOr(a.err, kErrTooLong);
-        return;
-    }
-    const int col0 = p.block * COLS, before = p.ctx - p.Lq;
+    const int before = p.ctx - p.Lq;
     const int min_pos = before + col0 / G; // the first column's, the least
     const int np = (before + min(p.Lq - 1, (col0 + COLS - 1) / G) + 16) >> 4, npr = (np + 1) >> 1;
     const int nw = npr > wave ? (npr - wave + UW - 1) / UW : 0; // this wave's pairs: wave, wave + UW, ...
@@ -242,6 +229,29 @@ __global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2,
     }
 }
 
+template <bool OUT_F32, int TILES, int UW>
+__global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2, 2))) varlenUnitKernel(UnitArgs a) {
+    // Parts of bf16 that a weight is summed in: 32-bit outputs hold 2^-24 of it,
+    // 16-bit ones of a tile 2^-16. Large batches with 16-bit outputs (TILES == 2)
+    // take one, 2^-9, which the output's own rounding is as large as: 3 chunks of
+    // 700 after 1500 tokens 42.1 -> 37.9 us.
+    constexpr int PARTS = OUT_F32 ? 3 : TILES == 2 ? 1 : 2;
+    // The last blocks first: they see the most keys of their sequence.
+    const int u = a.units - 1 - int(blockIdx.x);
+    const int h = u % a.nkvh;
+    Place p;
+    if (!placeOf(a, u / a.nkvh, 16 * TILES, p)) return;
+    if (!fits(p.q0, p.q0 + p.Lq, p.ctx, a)) {
+        if (threadIdx.x == 0) atomicOr(a.err, kErrTooLong);
+        return;
+    }
+    const int col0 = p.block * 16 * TILES;
+    // Where the second tile is empty, as a single query's is: 512 queries beside 200
+    // single ones 107 -> 103 us.
+    if (TILES == 2 && col0 + 16 >= p.Lq * a.G) return attendBlock<OUT_F32, 1, UW, PARTS>(a, p, h, col0);
+    attendBlock<OUT_F32, TILES, UW, PARTS>(a, p, h, col0);
+}
+
 } // namespace
 
 // By the number of workgroups that blocks of one tile make, at 12 query and 2 kv
@@ -249,7 +259,8 @@ __global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2,
 // last still with two parts of a weight):
 //   up to 256: 64 after 1900 tokens 25.8, 15.1, 13.5, 21.9; 64 after 8000 39.2,
 //     45.6, 39.4, 67.1; 256 after 8000 45.3, 47.2, 39.3, 69.6; 333 alone 22.6,
-//     7.1, 7.2, 9.7: 8 waves, which halve the walk over a long context
+//     7.1, 7.2, 9.7: 8 waves, which halve the walk over a long context, in
+//     tables of more than 64 pages
 //   up to 900: 777 alone 27.5, 12.8, 18.0, 14.3; 2 x 256 and 60 single queries
 //     25.7, 20.0, 23.9, 28.2; 1200 alone (902) 34.8, 19.7, 28.1, 19.4
 //   more: 4 x 1000 44.7, 50.7, 80.7, 41.9; 6 x 340 after 1700 50.4, 44.1, 54.6,
@@ -261,11 +272,13 @@ __global__ void __launch_bounds__(64 * UW) __attribute__((amdgpu_waves_per_eu(2,
 // ones up to 8000 182, 211; 4 x 256 after 6000 and 60 67, 76); beyond, a few
 // queries after 16000 tokens walk alone for 80 us.
 // Three and four tiles a block need one wave on a SIMD: 6 x 340 after 1700 55.6
-// and 61.0.
+// and 61.0. Blocks of one tile for the last round, to fill it: 4 x 512 after 4096
+// 67.7 -> 82.
 UnitShape unitShape(int B, int T, int nkvh, int group, int max_pages) {
     if (max_pages > 512) return {0, 0};
     const long long blocks = (((long long)T * group + 15) / 16 + B) * nkvh;
-    return blocks <= 256 ? UnitShape{1, 8} : blocks <= 900 ? UnitShape{1, 4} : UnitShape{2, 4};
+    if (blocks > 900) return {2, 4};
+    return {1, blocks <= 256 && max_pages > 64 ? 8 : 4};
 }
 
 void pagedVarlenUnits(void *out, bool out_f32, const uint16_t *q, const uint16_t *k_pool, const uint16_t *v_pool,

@@ -143,7 +143,7 @@ def test_chunks_long_and_many(dtype, qn, prior, extra):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("qn, prior, pages", [
     # on both sides of the lines between the kernels: 256 and 258 blocks of queries, 900 and 902
-    ([338], [0], 0), ([341], [0], 0), ([1197], [0], 0), ([1200], [0], 0), ([1100] + [1] * 90, [40] + [300] * 90, 0),
+    ([338], [0], 0), ([341], [0], 0), ([338], [0], 65), ([341], [0], 65), ([33], [991], 64), ([33], [992], 65), ([1197], [0], 0), ([1200], [0], 0), ([1100] + [1] * 90, [40] + [300] * 90, 0),
     # tables of 256 and 257 pages with 528 blocks, of 300 with 512 and 516, of 512 and 513 with few
     ([700], [3396], 256), ([700], [3397], 257), ([680], [33], 300), ([683], [33], 300), ([64], [8128], 512),
     ([64], [8129], 513), ([2, 1, 1, 70], [0, 0, 8191, 4000], 512),
