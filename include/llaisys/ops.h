@@ -178,7 +178,8 @@ __C {
      * the scale 2^E of each block and kv head: E the least whole number, -100 at
      * least, whose 448 * 2^E reaches the block's largest value. A value is read
      * back within 2^-4 of its size, or within 2^-10 * 2^E where that is more.
-     * Block tables are as for the bf16 pool.
+     * Block tables are as for the bf16 pool. Pools, rows, queries and outputs
+     * of these calls begin on 16 B boundaries.
      *
      * Append: row r of k_new, v_new [T, nkvh, 128] BF16 to slots[r] (I64, block
      * * 16 + offset, as llaisysPagedKVMap builds them; negative: the row is not
@@ -204,7 +205,10 @@ __C {
                                              llaisysTensor_t v_scale, llaisysTensor_t pairs);
     /* llaisysPagedAttention and llaisysPagedAttentionVarlen over the 8-bit pool:
      * the same arguments otherwise, with a positive scale; the softmax and the
-     * sums in 32 bits. */
+     * sums in 32 bits. Rows of a sequence that raises an error bit hold no
+     * result; rows that belong to no sequence are left as they were. Wide tables
+     * and batches take the runtime's workspace, which grows by allocation: under
+     * stream capture a call of the same sizes has to have run before. */
     __export void llaisysPagedAttentionF8(llaisysTensor_t out, llaisysTensor_t q, llaisysTensor_t k_pool,
                                           llaisysTensor_t v_pool, llaisysTensor_t k_scale, llaisysTensor_t v_scale,
                                           llaisysTensor_t block_table, llaisysTensor_t ctx_len, float scale);
@@ -225,7 +229,8 @@ __C {
      * * (in_scale[m] * weight_scale[n]) (+ bias[n], may be NULL), in [M, K] and
      * weight [N, K] I8, scales F32, out and bias F32, F16 or BF16. The products
      * are summed exactly in 32-bit integers (K <= 131071), the rest is 32-bit
-     * floats and one rounding. */
+     * floats and one rounding. Takes the runtime's workspace as llaisysLinear
+     * does. */
     __export void llaisysLinearI8(llaisysTensor_t out, llaisysTensor_t in, llaisysTensor_t in_scale,
                                   llaisysTensor_t weight, llaisysTensor_t weight_scale, llaisysTensor_t bias);
 }
