@@ -161,6 +161,25 @@ def test_chunks_at_the_lines(dtype, qn, prior, pages):
     check(got, want, most, cache, dtype, max(lens), True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nh, nkvh", [(12, 2), (3, 1)])
+@pytest.mark.parametrize("qn", [
+    [1] * 300,  # single queries only
+    [40, 1, 3] + [1] * 600, [2] * 1100 + [70], [1] * 3000 + [50], [300, 300] + [0] * 50 + [1] * 4000,
+])
+def test_many_sequences_over_wide_tables(dtype, nh, nkvh, qn):
+    """Past 512 pages, in batches that the work queue's tables hold, sort and do not."""
+    lens = [n + 7 * b % 40 for b, n in enumerate(qn)]
+    lens = [max(1, n) for n in lens]
+    lens[len(lens) // 2] += 900
+    cache, table, q = case(29, lens, nh, nkvh, qn, extra_pages=520, stale_nan=True)
+    got = varlen("amd", cache, table, q, np.concatenate([[0], np.cumsum(qn)]), lens, dtype)
+    assert L.device_error_flags() == 0
+    want, most = want_of(cache, table, lens, qn, q)
+    check(got, want, most, cache, dtype, max(lens), True)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("bad", [[60, 19, 33], [60, 1000, 33], [60, 0, 33]])  # too short, past the table, none
 @pytest.mark.parametrize("pages", [0, 600])

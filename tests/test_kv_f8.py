@@ -5,8 +5,8 @@ import pytest
 import torch
 
 import llaisys_amd as L
-from cases_8bit import (BAD_BLOCK, CODES, DEVICES, LEAST, TOO_LONG, Cache, bf16, encode64, exp_of, f64, give, table_of,
-                        take)
+from cases_8bit import (BAD_BLOCK, CODES, DEVICES, LEAST, TOO_LONG, Cache, attend64, bf16, encode64, exp_of, f64,
+                        give, table_of, take)
 
 
 def rows_of(seed, T, nkvh, spread=2.0):
@@ -216,6 +216,45 @@ def test_copied_blocks_grow_apart(device):
     cache.append(f64(k), f64(v), np.array([53, 21]))
     cache.check(*pools)
     assert (cache.exps[0][3] > cache.exps[0][1]).all()
+
+
+@pytest.mark.gpu
+def test_a_pool_of_more_than_4_gib():
+    """Append, block copy, gather and attention at both ends of it."""
+    blocks, nkvh, nh, lens = 1_100_000, 2, 12, [37, 50]
+    pools = [L.Tensor((blocks, nkvh, 16, 128), dtype=L.DataType.F8, device=L.DeviceType.AMD) for _ in range(2)]
+    pools += [L.Tensor((blocks, nkvh), dtype=L.DataType.F32, device=L.DeviceType.AMD) for _ in range(2)]
+    table = np.array([[blocks - 1, 3, blocks - 7, 0], [1_048_577, blocks - 30, 1_048_570, 12]], np.int32)
+    at = {int(b): i for i, b in enumerate(table.ravel())}
+    near = Cache(8, nkvh, 41)  # the same blocks, numbered from 0
+    k, v = rows_of(42, sum(lens), nkvh)
+    slots = slots_of(table, [0, 0], lens)
+    append("amd", pools, k, v, slots)
+    near.append(f64(k), f64(v), [at[int(x) // 16] * 16 + int(x) % 16 for x in slots])
+    q = bf16(np.random.RandomState(43).randn(2, nh, 128))
+    src = table.ravel()
+    pairs = np.stack([src, np.where(src > 2000, src - 300, src + 300)], 1)  # to blocks of no sequence
+    L.Ops.paged_kv_copy_blocks_f8(*pools, give(pairs.astype(np.int32), "amd"))
+    copied = np.array([[dict(pairs.tolist())[int(b)] for b in row] for row in table], np.int32)
+    for tab in (table, copied):
+        ko, vo = (give(torch.zeros(sum(lens), nkvh, 128, dtype=torch.bfloat16), "amd") for _ in range(2))
+        L.Ops.paged_kv_gather_f8(ko, vo, *pools, give(tab, "amd"), give(np.array([0, 37, 87], np.int32), "amd"))
+        outs = [give(torch.zeros(q.shape, dtype=torch.float32), "amd") for _ in range(2)]
+        ctx = give(np.array(lens, np.int32), "amd")
+        L.Ops.paged_attention_f8(outs[0], give(q, "amd"), *pools, give(tab, "amd"), ctx, 128 ** -0.5)
+        L.Ops.paged_attention_varlen_f8(outs[1], give(q, "amd"), *pools, give(tab, "amd"),
+                                        give(np.array([0, 1, 2], np.int32), "amd"), ctx, 128 ** -0.5)
+        assert L.device_error_flags() == 0
+        for b, n in enumerate(lens):
+            K, V = (near.values(w).reshape(2, 4, nkvh, 16, 128)[b].transpose(0, 2, 1, 3).reshape(64, nkvh, 128)[:n]
+                    for w in range(2))
+            r = slice(37 * b, 37 * b + n)
+            np.testing.assert_array_equal(take(ko)[r].double().numpy(), K)
+            np.testing.assert_array_equal(take(vo)[r].double().numpy(), V)
+            want, most = attend64(f64(q[b:b + 1]), K, V, 128 ** -0.5)
+            bound = np.abs(V).max() * (2 * 130 * 2.0 ** -24 * most + 2.0 ** -16 + 64 * 2.0 ** -24)
+            for o in outs:
+                assert np.abs(take(o)[b].double().numpy() - want[0]).max() <= bound + 2.0 ** -24 * np.abs(want).max()
 
 
 def test_the_plain_form_itself():
