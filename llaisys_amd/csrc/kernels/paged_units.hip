@@ -83,6 +83,30 @@ __device__ bool placeOf(const UnitArgs &a, int index, int columns, Place &p) {
     return false;
 }
 
+// softmaxUpdate with weights of one bf16 part, whose sum the matrix cores take as
+// rounded (a row of ones beside V): the rounding moves the quotient's two sides
+// alike, and the vector unit is the one that has no time (8000 queries alone 231 ->
+// 226 us).
+__device__ __forceinline__ void weightsOnce(Acc &acc, f32x4 &sum, const float (&sv)[8], PairP<1> &P, float scale_log2) {
+    constexpr float kLazyLog2 = 8.f;
+    float most = sv[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, sv[i]);
+    if (__builtin_amdgcn_ballot_w64(most * scale_log2 > acc.m + kLazyLog2) != 0) {
+        const float m = fmaxf(acc.m, maxOverGroups(most) * scale_log2);
+        const float alpha = exp2Fast(acc.m - (m == -INFINITY ? 0.f : m));
+        sum *= alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc.o[i] *= alpha;
+        acc.m = m;
+    }
+    const float m_use = acc.m == -INFINITY ? 0.f : acc.m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) P.part[0][i] = (__bf16)exp2Fast(__builtin_fmaf(sv[i], scale_log2, -m_use));
+    const uint32_t one = 0x3f803f80u;
+    sum = mfma::mfma(asBf16(u32x4{one, one, one, one}), P.part[0], sum);
+}
+
 // The 16 TILES columns from col0 on, of kv head h.
 template <bool OUT_F32, int TILES, int UW, int PARTS>
 __device__ __forceinline__ void attendBlock(const UnitArgs &a, const Place &p, int h, int col0) {
@@ -138,8 +162,12 @@ __device__ __forceinline__ void attendBlock(const UnitArgs &a, const Place &p, i
                    (size_t(bB) * a.nkvh + h) * KvF8::kPageVecs);
     };
     Acc acc[TILES];
+    f32x4 sums[TILES]; // of weights of one part
 #pragma unroll
-    for (int k = 0; k < TILES; ++k) acc[k].reset();
+    for (int k = 0; k < TILES; ++k) {
+        acc[k].reset();
+        sums[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     for (; base < nw; base += WINDOW) {
         cnt = min(WINDOW, nw - base);
         if (base != 0) loadWindow();
@@ -174,9 +202,13 @@ __device__ __forceinline__ void attendBlock(const UnitArgs &a, const Place &p, i
                     PairP<PARTS> P[TILES];
 #pragma unroll
                     for (int k = 0; k < TILES; ++k) {
-                        const float(&s1)[1][8] = *reinterpret_cast<const float(*)[1][8]>(&sv[k]);
-                        PairP<PARTS>(&p1)[1] = *reinterpret_cast<PairP<PARTS>(*)[1]>(&P[k]);
-                        softmaxUpdate<PARTS, 1>(acc[k], s1, p1, a.scale_log2);
+                        if constexpr (PARTS == 1) {
+                            weightsOnce(acc[k], sums[k], sv[k], P[k], a.scale_log2);
+                        } else {
+                            const float(&s1)[1][8] = *reinterpret_cast<const float(*)[1][8]>(&sv[k]);
+                            PairP<PARTS>(&p1)[1] = *reinterpret_cast<PairP<PARTS>(*)[1]>(&P[k]);
+                            softmaxUpdate<PARTS, 1>(acc[k], s1, p1, a.scale_log2);
+                        }
                     }
                     u32x4 va[4], vb[4];
 #pragma unroll
@@ -197,8 +229,11 @@ __device__ __forceinline__ void attendBlock(const UnitArgs &a, const Place &p, i
     // tile, until wave 0 has it all.
 #pragma unroll
     for (int k = 0; k < TILES; ++k) {
-        float L = acc[k].l + __shfl_xor(acc[k].l, 16), M = acc[k].m;
-        L += __shfl_xor(L, 32);
+        float L = sums[k][0], M = acc[k].m;
+        if constexpr (PARTS > 1) {
+            L = acc[k].l + __shfl_xor(acc[k].l, 16);
+            L += __shfl_xor(L, 32);
+        }
 #pragma unroll
         for (int half = UW / 2; half > 0; half /= 2) {
             if (k > 0 || half < UW / 2) __syncthreads(); // the states before have been read
