@@ -17,7 +17,7 @@
 // some 400 cycles per page pair) and rounding beside 256 cycles of matrix
 // instructions, on two waves a SIMD. 12 query and 2 kv heads, us, here and the
 // persistent kernel: a chunk of 777 queries 12.8, 27.5; 4 chunks of 512 after
-// 4096 tokens beside 60 single queries 68.4, 77.9.
+// 4096 tokens beside 60 single queries 66.0, 77.9.
 //
 // Consecutive workgroups take the kv heads in turn, as consecutive workgroups go
 // to the XCDs in turn: where the heads divide the 8 XCDs, an XCD's L2 holds the
