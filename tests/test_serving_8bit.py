@@ -5,6 +5,7 @@ stage is compared with its 64-bit form on what the stage before it gave, and the
 cache with a cache that the host kept; then the same on another stream and
 captured into a graph."""
 import contextlib
+import threading
 from types import SimpleNamespace
 
 import numpy as np
@@ -208,3 +209,29 @@ def test_captured_steps_replayed(rows, width):
                     new[r.randint(B)] += r.randint(rows - B + 1)
                     new[r.randint(B)] = 0
                 step(run, 2, 100 + i, new, lambda state, s: run[4].replay())
+
+
+@pytest.mark.gpu
+def test_steps_on_two_threads_at_once():
+    """Each thread has a runtime, a stream and a workspace of its own."""
+    def serve(seed, failures):
+        try:
+            layer = Layer("amd", seed)
+            for turn in range(4):
+                state, before = layer.state(4, 600 if turn % 2 else WIDTH), begin(4, 600 if turn % 2 else WIDTH)
+                for i, new in enumerate(([40, 1, 7, 20], [1, 1, 1, 1], [1, 30, 2, 1], [1, 1, 1, 1])):
+                    s = layer.step(4, sum(new))
+                    fill(s["x"], bf16(np.random.RandomState(seed + i).randn(s["T"], HIDDEN)))
+                    fill(s["new"], torch.tensor(new, dtype=torch.int32))
+                    layer.run(state, s)
+                    before = layer.check_step(state, s, before, new)
+        except BaseException as e:  # noqa: BLE001 (reported by the test's own thread)
+            failures.append(e)
+
+    failures = []
+    threads = [threading.Thread(target=serve, args=(seed, failures)) for seed in (51, 52)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
